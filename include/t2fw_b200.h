@@ -284,6 +284,68 @@ int t2fw_selftest_umma16(const float *A1, const float *B1, const float *A2, cons
                          float *D1, float *D2, int N, int Kc, int a_mn, int b_mn, int *status,
                          void *stream);
 
+/* ---- operators that stand around the recurrences in a model; none has a counterpart in the reference ---- */
+
+/*
+ * Gated linear recurrence with a state of one number per channel:
+ *
+ *   h_t = forget_t h_{t-1} + value_t ,  outputs_t = h_t ,  next_state = h_T
+ *
+ * value, forget, outputs and their gradients [B, T, D]; state, next_state and their gradients [B, D].  Every dtype, any
+ * sizes, element-aligned pointers.  The gates are taken as given.  Long sequences are worked on in parts, between which the
+ * products of the gates over a part (fp32; fp64 for fp64 storage) carry the state: where such a product leaves the range
+ * of its type upwards while the state it meets is no zero, the result is infinite or NaN, which a step-by-step evaluation
+ * of gates above 1 reaches soon after.
+ * grad_state may be NULL (zero).
+ */
+int t2fw_glr_forward(const void *value, const void *forget, const void *state, void *outputs, void *next_state, int64_t B,
+                     int64_t T, int64_t D, int dtype, void *stream);
+int t2fw_glr_backward(const void *grad_output, const void *grad_state, const void *forget, const void *outputs,
+                      const void *state, void *d_value, void *d_forget, void *d_state, int64_t B, int64_t T, int64_t D,
+                      int dtype, void *stream);
+
+/*
+ * The same as a layer core on a projection output vg [B, T, 2*D] = value | gate pre-activation, read in place:
+ * a = sigmoid(gate), h_t = a_t h_{t-1} + (1 - a_t) value_t.  d_vg has vg's layout.
+ */
+int t2fw_glr_fused_forward(const void *vg, const void *state, void *outputs, void *next_state, int64_t B, int64_t T,
+                           int64_t D, int dtype, void *stream);
+int t2fw_glr_fused_backward(const void *grad_output, const void *grad_state, const void *vg, const void *outputs,
+                            const void *state, void *d_vg, void *d_state, int64_t B, int64_t T, int64_t D, int dtype,
+                            void *stream);
+
+/*
+ * Root-mean-square norm of `rows` rows of D, with the residual's addition where `residual` is given:
+ *
+ *   s = x + residual ,  y = s / sqrt(mean(s^2) + eps) * weight ,  sum = s
+ *
+ * residual and sum are NULL together.  y is computed from s before its rounding to the storage type.  The 8-bit form
+ * writes q = e4m3(y / scale), rounded to nearest, and one fp32 scale = max(max|y| / 448, 1e-30) per row; no fp64.
+ * Backward: `s` is what the forward call left in `sum` (x without a residual); d_s is the gradient of x and of the
+ * residual alike; grad_sum, the gradient of `sum` from its other uses, may be NULL (zero).
+ */
+int t2fw_rms_norm_forward(const void *x, const void *residual, const void *weight, void *y, void *sum, int64_t rows,
+                          int64_t D, double eps, int dtype, void *stream);
+int t2fw_rms_norm_e4m3(const void *x, const void *residual, const void *weight, void *q, float *scale, void *sum,
+                       int64_t rows, int64_t D, double eps, int dtype, void *stream);
+size_t t2fw_rms_norm_backward_scratch_bytes(int64_t rows, int64_t D, int dtype);
+int t2fw_rms_norm_backward(const void *grad_y, const void *grad_sum, const void *s, const void *weight, void *d_s,
+                           void *d_weight, int64_t rows, int64_t D, double eps, int dtype, void *scratch,
+                           size_t scratch_bytes, void *stream);
+
+/*
+ * Global norm of n tensors, total = sqrt(sum of all squares), and clipping by it: out = c * tensor with
+ * c = min(1, max_norm / (total + 1e-6)).  The lists are HOST arrays of device addresses, element counts (positive) and
+ * dtypes, which may differ; the tensors are dense.  total is one device number, fp32 or fp64.  out[i] == tensors[i] for
+ * all i scales in place (nothing is written where c = 1; the tensors must not overlap), else the outputs overlap no input.
+ * Sums are kept in fp64; a total that is infinite or NaN goes into c as it is.
+ */
+size_t t2fw_grad_clip_scratch_bytes(int64_t n_tensors);
+int t2fw_grad_norm(const void *const *tensors, const int64_t *numel, const int *dtype, int64_t n, void *total,
+                   int total_dtype, void *scratch, size_t scratch_bytes, void *stream);
+int t2fw_grad_clip(const void *const *tensors, void *const *out, const int64_t *numel, const int *dtype, int64_t n,
+                   double max_norm, void *total, int total_dtype, void *scratch, size_t scratch_bytes, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

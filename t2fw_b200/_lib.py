@@ -1,7 +1,7 @@
 """Loading of the two native libraries.
 
   load_core() -> ctypes.CDLL of libt2fw_b200.so, the C ABI declared in include/t2fw_b200.h
-  load_ops()  -> registers torch.ops.lfw / torch.ops.dfw from t2fw_torch_ops.so
+  load_ops()  -> registers torch.ops.lfw / dfw / glr / rms / gradclip from t2fw_torch_ops.so
 
 Both fail loudly (ImportError) when the library has not been built: nothing falls back to a
 slower path.
@@ -26,6 +26,9 @@ EXPORTS = (
     "t2fw_dfw_backward_noalloc_max_elems", "t2fw_dfw_backward_noalloc",
     "t2fw_lfw_fused_scratch_bytes", "t2fw_lfw_fused_forward", "t2fw_lfw_fused_backward",
     "t2fw_lfw_segment_summary_scratch_bytes", "t2fw_lfw_segment_summary", "t2fw_lfw_fold_summaries",
+    "t2fw_glr_forward", "t2fw_glr_backward", "t2fw_glr_fused_forward", "t2fw_glr_fused_backward",
+    "t2fw_rms_norm_forward", "t2fw_rms_norm_e4m3", "t2fw_rms_norm_backward", "t2fw_rms_norm_backward_scratch_bytes",
+    "t2fw_grad_norm", "t2fw_grad_clip", "t2fw_grad_clip_scratch_bytes",
 )
 
 _core = None
@@ -35,6 +38,7 @@ _i64 = ctypes.c_int64
 _vp = ctypes.c_void_p
 _int = ctypes.c_int
 _sz = ctypes.c_size_t
+_f64 = ctypes.c_double
 
 
 def load_core():
@@ -85,12 +89,34 @@ def load_core():
     lib.t2fw_lfw_fused_forward.argtypes = [_vp] * 4 + [_i64] * 3 + [_int, _vp, _sz, _vp]
     lib.t2fw_lfw_fused_backward.restype = _int
     lib.t2fw_lfw_fused_backward.argtypes = [_vp] * 7 + [_i64] * 3 + [_int, _vp, _sz, _vp]
+    lib.t2fw_glr_forward.restype = _int
+    lib.t2fw_glr_forward.argtypes = [_vp] * 5 + [_i64] * 3 + [_int, _vp]
+    lib.t2fw_glr_backward.restype = _int
+    lib.t2fw_glr_backward.argtypes = [_vp] * 8 + [_i64] * 3 + [_int, _vp]
+    lib.t2fw_glr_fused_forward.restype = _int
+    lib.t2fw_glr_fused_forward.argtypes = [_vp] * 4 + [_i64] * 3 + [_int, _vp]
+    lib.t2fw_glr_fused_backward.restype = _int
+    lib.t2fw_glr_fused_backward.argtypes = [_vp] * 7 + [_i64] * 3 + [_int, _vp]
+    lib.t2fw_rms_norm_forward.restype = _int
+    lib.t2fw_rms_norm_forward.argtypes = [_vp] * 5 + [_i64] * 2 + [_f64, _int, _vp]
+    lib.t2fw_rms_norm_e4m3.restype = _int
+    lib.t2fw_rms_norm_e4m3.argtypes = [_vp] * 6 + [_i64] * 2 + [_f64, _int, _vp]
+    lib.t2fw_rms_norm_backward_scratch_bytes.restype = _sz
+    lib.t2fw_rms_norm_backward_scratch_bytes.argtypes = [_i64, _i64, _int]
+    lib.t2fw_rms_norm_backward.restype = _int
+    lib.t2fw_rms_norm_backward.argtypes = [_vp] * 6 + [_i64] * 2 + [_f64, _int, _vp, _sz, _vp]
+    lib.t2fw_grad_clip_scratch_bytes.restype = _sz
+    lib.t2fw_grad_clip_scratch_bytes.argtypes = [_i64]
+    lib.t2fw_grad_norm.restype = _int
+    lib.t2fw_grad_norm.argtypes = [_vp] * 3 + [_i64, _vp, _int, _vp, _sz, _vp]
+    lib.t2fw_grad_clip.restype = _int
+    lib.t2fw_grad_clip.argtypes = [_vp] * 4 + [_i64, _f64, _vp, _int, _vp, _sz, _vp]
     _core = lib
     return lib
 
 
 def load_ops():
-    """Registers torch.ops.lfw / torch.ops.dfw and returns the extension module with the autograd entry points."""
+    """Registers torch.ops.lfw / dfw / glr / rms / gradclip and returns the extension module with the autograd entry points."""
     global _ops
     if _ops is not None:
         return _ops
@@ -109,7 +135,7 @@ def load_ops():
 
 
 # which of set_fallback()'s slots belongs to which class
-LFW, DFW, FUSED = range(3)
+LFW, DFW, FUSED, GLR, GLR_FUSED, RMS, ADD_RMS = range(7)
 
 
 def bind_apply(cls, which, native):

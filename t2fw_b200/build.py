@@ -1,7 +1,7 @@
 """Ahead-of-time build of the native libraries, in-tree.
 
   lib/libt2fw_b200.so     CUDA kernels + the C ABI (include/t2fw_b200.h); nvcc, sm_100a only
-  lib/t2fw_torch_ops.so   the PyTorch operator library (torch.ops.lfw / torch.ops.dfw), a thin
+  lib/t2fw_torch_ops.so   the PyTorch operator library (torch.ops.lfw / dfw / glr / rms / gradclip), a thin
                           C++ adapter that links against the former; also the Python extension
                           module with the autograd entry points
 
@@ -79,8 +79,9 @@ def build_ops(force=False, verbose=False):
     import torch
     from torch.utils import cpp_extension
 
-    srcs = [os.path.join(CSRC, "torch_ops.cpp"), os.path.join(CSRC, "torch_bind.cpp")]
-    deps = srcs + [os.path.join(CSRC, "torch_ops.h"), os.path.join(ROOT, "include", "t2fw_b200.h")]
+    srcs = [os.path.join(CSRC, n) for n in ("torch_ops.cpp", "torch_layer_ops.cpp", "torch_bind.cpp")]
+    deps = srcs + [os.path.join(CSRC, n) for n in ("torch_ops.h", "torch_util.h")] + \
+        [os.path.join(ROOT, "include", "t2fw_b200.h")]
     if not force and _newer(OPS_LIB, deps) and _newer(OPS_LIB, [CORE_LIB]):
         return OPS_LIB
     tlib = os.path.join(os.path.dirname(torch.__file__), "lib")

@@ -214,4 +214,27 @@ int dfw_scan_backward(const void *go, const void *gs, const void *q, const void 
                       void *dv_acc, int64_t B, int64_t T, int64_t D, int64_t M, int dtype,
                       cudaStream_t st);
 
+// gated linear recurrence with a state of one number per channel (glr.cu); gs may be null (zero)
+int glr_step(const void *x, const void *f, const void *state, void *out, void *next, int64_t n, int dtype, cudaStream_t st);
+int glr_forward(const void *x, const void *f, const void *state, void *out, void *next, int64_t B, int64_t T, int64_t D,
+                int dtype, cudaStream_t st);
+int glr_fused_forward(const void *vg, const void *state, void *out, void *next, int64_t B, int64_t T, int64_t D, int dtype,
+                      cudaStream_t st);
+int glr_backward(const void *go, const void *gs, const void *f, const void *out, const void *state, void *dx, void *df,
+                 void *ds, int64_t B, int64_t T, int64_t D, int dtype, cudaStream_t st);
+int glr_fused_backward(const void *go, const void *gs, const void *vg, const void *out, const void *state, void *dvg,
+                       void *ds, int64_t B, int64_t T, int64_t D, int dtype, cudaStream_t st);
+// root-mean-square norm (rms_norm.cu); r and sum are null together, dsum may be null (zero)
+int rms_norm_forward(const void *x, const void *r, const void *w, void *y, void *sum, int64_t rows, int64_t D, double eps,
+                     int dtype, cudaStream_t st);
+int rms_norm_e4m3(const void *x, const void *r, const void *w, void *q, float *scale, void *sum, int64_t rows, int64_t D,
+                  double eps, int dtype, cudaStream_t st);
+size_t rms_norm_backward_scratch_bytes(int64_t rows, int64_t D, int dtype);
+int rms_norm_backward(const void *dy, const void *dsum, const void *s, const void *w, void *ds, void *dw, int64_t rows,
+                      int64_t D, double eps, int dtype, void *scratch, cudaStream_t st);
+// global norm of n tensors and scaling by it (grad_clip.cu); max_norm < 0: only the norm, out unused
+size_t grad_clip_scratch_bytes(int64_t n);
+int grad_clip(const void *const *in, void *const *out, const int64_t *numel, const int *dtype, int n, double max_norm,
+              void *total, int total_dtype, void *scratch, cudaStream_t st);
+
 }  // namespace t2fw

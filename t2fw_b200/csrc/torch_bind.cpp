@@ -1,6 +1,6 @@
-// Python binding of the autograd entry points: LFWFunction.apply, DFWFunction.apply,
-// LFWFusedFunction.apply and lfw_decode_step as C functions of the extension module that this library
-// also is.
+// Python binding of the entry points that a small call spends its time in: the apply of the autograd classes
+// (LFWFunction, DFWFunction, LFWFusedFunction, GLRFunction, GLRFusedFunction, RMSNormFunction, AddRMSNormFunction), the
+// decode steps, the 8-bit norm and gradient clipping as C functions of the extension module that this library also is.
 //
 // Why: a call on a small problem is bound by the host.  Through a Python autograd function and torch.ops
 // one token of 32 rows cost 18 us of host time around a 3 us kernel, and a backward pass had to wait for
@@ -104,8 +104,74 @@ struct FusedNode : torch::autograd::Function<FusedNode> {
   }
 };
 
+// The gradient of an output that nothing used stays undefined here: the kernels take its absence as zero where they can.
+struct GlrNode : torch::autograd::Function<GlrNode> {
+  static variable_list forward(AutogradContext *ctx, const Tensor &x, const Tensor &f, const Tensor &s) {
+    auto r = t2fw_ops::glr_forward(x, f, s);
+    ctx->set_materialize_grads(false);
+    ctx->save_for_backward({f, r[0], s});
+    return r;
+  }
+  static variable_list backward(AutogradContext *ctx, variable_list g) {
+    const auto v = ctx->get_saved_variables();
+    const Tensor go = g[0].defined() ? g[0].contiguous() : at::zeros_like(v[1]);
+    return no_second_derivative(
+        t2fw_ops::glr_backward(go, g[1].defined() ? g[1].contiguous() : Tensor(), v[0], v[1], v[2]), g, v);
+  }
+};
+
+struct GlrFusedNode : torch::autograd::Function<GlrFusedNode> {
+  static variable_list forward(AutogradContext *ctx, const Tensor &vg, const Tensor &s) {
+    auto r = t2fw_ops::glr_fused_forward(vg, s);
+    ctx->set_materialize_grads(false);
+    ctx->save_for_backward({vg, r[0], s});
+    return r;
+  }
+  static variable_list backward(AutogradContext *ctx, variable_list g) {
+    const auto v = ctx->get_saved_variables();
+    const Tensor go = g[0].defined() ? g[0].contiguous() : at::zeros_like(v[1]);
+    return no_second_derivative(
+        t2fw_ops::glr_fused_backward(go, g[1].defined() ? g[1].contiguous() : Tensor(), v[0], v[1], v[2]), g, v);
+  }
+};
+
+struct RmsNode : torch::autograd::Function<RmsNode> {
+  static variable_list forward(AutogradContext *ctx, const Tensor &x, const Tensor &w, double eps) {
+    auto r = t2fw_ops::rms_forward(x, std::nullopt, w, eps);
+    ctx->save_for_backward({x, w});
+    ctx->saved_data["eps"] = eps;
+    return r;
+  }
+  static variable_list backward(AutogradContext *ctx, variable_list g) {
+    const auto v = ctx->get_saved_variables();
+    auto r = no_second_derivative(
+        t2fw_ops::rms_backward(g[0].contiguous(), std::nullopt, v[0], v[1], ctx->saved_data["eps"].toDouble()), g, v);
+    return {r[0], r[1], Tensor()};
+  }
+};
+
+struct AddRmsNode : torch::autograd::Function<AddRmsNode> {
+  static variable_list forward(AutogradContext *ctx, const Tensor &x, const Tensor &res, const Tensor &w, double eps) {
+    auto r = t2fw_ops::rms_forward(x, res, w, eps);
+    ctx->set_materialize_grads(false);
+    ctx->save_for_backward({r[1], w});
+    ctx->saved_data["eps"] = eps;
+    return r;
+  }
+  static variable_list backward(AutogradContext *ctx, variable_list g) {
+    const auto v = ctx->get_saved_variables();
+    const Tensor gy = g[0].defined() ? g[0].contiguous() : at::zeros_like(v[0]);
+    auto r = no_second_derivative(t2fw_ops::rms_backward(gy, g[1].defined() ? g[1].contiguous() : Tensor(), v[0], v[1],
+                                                         ctx->saved_data["eps"].toDouble()), g, v);
+    return {r[0], r[0], r[1], Tensor()};      // one gradient for both, as the gradient of a sum is
+  }
+};
+
 // ---- argument handling --------------------------------------------------------------------------
-PyObject *g_fallback[3] = {nullptr, nullptr, nullptr};      // Python's LFWFunction / DFWFunction / LFWFusedFunction apply
+// the Python classes' apply: LFWFunction, DFWFunction, LFWFusedFunction, GLRFunction, GLRFusedFunction, RMSNormFunction,
+// AddRMSNormFunction
+constexpr int kClasses = 7;
+PyObject *g_fallback[kClasses] = {};
 
 PyObject *call_fallback(int which, PyObject *const *args, Py_ssize_t n) {
   if (g_fallback[which] == nullptr) {
@@ -273,6 +339,184 @@ PyObject *py_decode_ring(PyObject *, PyObject *const *args, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
+// Whether every argument is a plain tensor of the first one's type.
+bool plain_args(PyObject *const *args, int n) {
+  for (int i = 0; i < n; ++i)
+    if (!plain_tensor(args[i]) || THPVariable_Unpack(args[i]).scalar_type() != THPVariable_Unpack(args[0]).scalar_type())
+      return false;
+  return plain_mode();
+}
+
+PyObject *tuple_to_python(std::vector<Tensor> r) {
+  THPObjectPtr tup(PyTuple_New((Py_ssize_t)r.size()));
+  if (!tup) throw python_error();
+  for (size_t i = 0; i < r.size(); ++i) PyTuple_SET_ITEM(tup.get(), (Py_ssize_t)i, THPVariable_Wrap(std::move(r[i])));
+  return tup.release();
+}
+
+PyObject *py_glr_apply(PyObject *, PyObject *const *args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (n == 3 && plain_args(args, 3)) {
+    const Tensor &x = THPVariable_Unpack(args[0]), &f = THPVariable_Unpack(args[1]), &s = THPVariable_Unpack(args[2]);
+    if (x.sizes() == f.sizes()) {
+      const Tensor *all[3] = {&x, &f, &s};
+      std::vector<Tensor> r;
+      {
+        pybind11::gil_scoped_release no_gil;
+        r = any_requires_grad(all, 3) ? GlrNode::apply(x, f, s) : t2fw_ops::glr_forward(x, f, s);
+      }
+      return tuple_to_python(std::move(r));
+    }
+  }
+  return call_fallback(3, args, n);
+  END_HANDLE_TH_ERRORS
+}
+
+PyObject *py_glr_fused_apply(PyObject *, PyObject *const *args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (n == 2 && plain_args(args, 2)) {
+    const Tensor &vg = THPVariable_Unpack(args[0]), &s = THPVariable_Unpack(args[1]);
+    if (vg.dim() == 3 && s.dim() == 2 && vg.size(2) % 2 == 0 && s.size(0) == vg.size(0) && s.size(1) == vg.size(2) / 2 &&
+        vg.is_contiguous() && s.is_contiguous()) {
+      const Tensor *all[2] = {&vg, &s};
+      std::vector<Tensor> r;
+      {
+        pybind11::gil_scoped_release no_gil;
+        r = any_requires_grad(all, 2) ? GlrFusedNode::apply(vg, s) : t2fw_ops::glr_fused_forward(vg, s);
+      }
+      return tuple_to_python(std::move(r));
+    }
+  }
+  return call_fallback(4, args, n);
+  END_HANDLE_TH_ERRORS
+}
+
+// Whether the norm's arguments (x, [residual,] weight, eps) are the plain case.
+bool plain_norm(PyObject *const *args, Py_ssize_t n, int tensors) {
+  if (n != tensors + 1 || !PyFloat_CheckExact(args[tensors]) || !plain_args(args, tensors)) return false;
+  const Tensor &x = THPVariable_Unpack(args[0]), &w = THPVariable_Unpack(args[tensors - 1]);
+  if (x.dim() < 1 || w.dim() != 1 || x.size(-1) != w.size(0) || !x.is_contiguous() || !w.is_contiguous()) return false;
+  if (tensors == 3) {
+    const Tensor &r = THPVariable_Unpack(args[1]);
+    if (r.sizes() != x.sizes() || !r.is_contiguous()) return false;
+  }
+  return PyFloat_AS_DOUBLE(args[tensors]) >= 0;
+}
+
+PyObject *py_rms_apply(PyObject *, PyObject *const *args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (plain_norm(args, n, 2)) {
+    const Tensor &x = THPVariable_Unpack(args[0]), &w = THPVariable_Unpack(args[1]);
+    const double eps = PyFloat_AS_DOUBLE(args[2]);
+    const Tensor *all[2] = {&x, &w};
+    std::vector<Tensor> r;
+    {
+      pybind11::gil_scoped_release no_gil;
+      r = any_requires_grad(all, 2) ? RmsNode::apply(x, w, eps) : t2fw_ops::rms_forward(x, std::nullopt, w, eps);
+    }
+    return THPVariable_Wrap(std::move(r[0]));
+  }
+  return call_fallback(5, args, n);
+  END_HANDLE_TH_ERRORS
+}
+
+PyObject *py_add_rms_apply(PyObject *, PyObject *const *args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (plain_norm(args, n, 3)) {
+    const Tensor &x = THPVariable_Unpack(args[0]), &res = THPVariable_Unpack(args[1]), &w = THPVariable_Unpack(args[2]);
+    const double eps = PyFloat_AS_DOUBLE(args[3]);
+    const Tensor *all[3] = {&x, &res, &w};
+    std::vector<Tensor> r;
+    {
+      pybind11::gil_scoped_release no_gil;
+      r = any_requires_grad(all, 3) ? AddRmsNode::apply(x, res, w, eps) : t2fw_ops::rms_forward(x, res, w, eps);
+    }
+    return tuple_to_python(std::move(r));
+  }
+  return call_fallback(6, args, n);
+  END_HANDLE_TH_ERRORS
+}
+
+// rms_e4m3(x, residual or None, weight, eps): a tuple, or NotImplemented if this is not the plain case
+PyObject *py_rms_e4m3(PyObject *, PyObject *const *args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (n != 4) Py_RETURN_NOTIMPLEMENTED;
+  const bool add = args[1] != Py_None;
+  PyObject *const plain[4] = {args[0], add ? args[1] : args[2], add ? args[2] : args[3], args[3]};
+  if (!plain_norm(plain, add ? 4 : 3, add ? 3 : 2)) Py_RETURN_NOTIMPLEMENTED;
+  const Tensor &x = THPVariable_Unpack(args[0]), &w = THPVariable_Unpack(args[2]);
+  const std::optional<Tensor> res = add ? std::optional<Tensor>(THPVariable_Unpack(args[1])) : std::nullopt;
+  const Tensor *all[3] = {&x, &w, add ? &*res : &w};
+  if (any_requires_grad(all, 3)) Py_RETURN_NOTIMPLEMENTED;
+  const double eps = PyFloat_AS_DOUBLE(args[3]);
+  std::vector<Tensor> r;
+  {
+    pybind11::gil_scoped_release no_gil;
+    r = t2fw_ops::rms_e4m3(x, res, w, eps);
+  }
+  return tuple_to_python(std::move(r));
+  END_HANDLE_TH_ERRORS
+}
+
+// glr_step(value, forget, state_in, state_out, outputs): None, or NotImplemented as decode_step
+PyObject *py_glr_step(PyObject *, PyObject *const *args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (n != 5 || !plain_args(args, 5)) Py_RETURN_NOTIMPLEMENTED;
+  const Tensor *t[5];
+  for (int i = 0; i < 5; ++i) t[i] = &THPVariable_Unpack(args[i]);
+  {
+    pybind11::gil_scoped_release no_gil;
+    t2fw_ops::glr_decode_step(*t[0], *t[1], *t[2], *t[3], *t[4]);
+  }
+  Py_RETURN_NONE;
+  END_HANDLE_TH_ERRORS
+}
+
+// The tensors of a list; false if it holds anything but plain ones.
+bool plain_list(PyObject *l, std::vector<Tensor> &out) {
+  if (!PyList_CheckExact(l) || !plain_mode()) return false;
+  const Py_ssize_t n = PyList_GET_SIZE(l);
+  out.reserve((size_t)n);
+  for (Py_ssize_t i = 0; i < n; ++i) {
+    PyObject *o = PyList_GET_ITEM(l, i);
+    if (!plain_tensor(o)) return false;
+    out.push_back(THPVariable_Unpack(o));
+  }
+  return n > 0;
+}
+
+// grad_clip(list, max_norm, in_place): total, or (total, clipped list); NotImplemented if this is not the plain case
+PyObject *py_grad_clip(PyObject *, PyObject *const *args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  std::vector<Tensor> l;
+  if (n != 3 || !PyFloat_CheckExact(args[1]) || !plain_list(args[0], l)) Py_RETURN_NOTIMPLEMENTED;
+  const double max_norm = PyFloat_AS_DOUBLE(args[1]);
+  if (args[2] == Py_True) {
+    Tensor total;
+    {
+      pybind11::gil_scoped_release no_gil;
+      total = t2fw_ops::grad_clip_(l, max_norm);
+    }
+    return THPVariable_Wrap(std::move(total));
+  }
+  for (const Tensor &t : l)
+    if (t.requires_grad() && at::GradMode::is_enabled()) Py_RETURN_NOTIMPLEMENTED;
+  std::vector<Tensor> r;
+  {
+    pybind11::gil_scoped_release no_gil;
+    r = t2fw_ops::grad_clip(l, max_norm);
+  }
+  THPObjectPtr list(PyList_New((Py_ssize_t)r.size() - 1));
+  if (!list) throw python_error();
+  for (size_t i = 1; i < r.size(); ++i) PyList_SET_ITEM(list.get(), (Py_ssize_t)i - 1, THPVariable_Wrap(std::move(r[i])));
+  THPObjectPtr tup(PyTuple_New(2));
+  if (!tup) throw python_error();
+  PyTuple_SET_ITEM(tup.get(), 0, THPVariable_Wrap(std::move(r[0])));
+  PyTuple_SET_ITEM(tup.get(), 1, list.release());
+  return tup.release();
+  END_HANDLE_TH_ERRORS
+}
+
 // no_second_derivative(gradients, upstream and saved tensors) -> gradients: for the Python classes
 PyObject *py_no_second_derivative(PyObject *, PyObject *const *args, Py_ssize_t n) {
   HANDLE_TH_ERRORS
@@ -293,10 +537,10 @@ PyObject *py_no_second_derivative(PyObject *, PyObject *const *args, Py_ssize_t 
   END_HANDLE_TH_ERRORS
 }
 
-// set_fallback(which, callable): 0 LFWFunction, 1 DFWFunction, 2 LFWFusedFunction
+// set_fallback(which, callable): the classes in g_fallback's order
 PyObject *py_set_fallback(PyObject *, PyObject *const *args, Py_ssize_t n) {
   const long w = n == 2 ? PyLong_AsLong(args[0]) : -1;
-  if (w < 0 || w > 2 || !PyCallable_Check(args[1])) {
+  if (w < 0 || w >= kClasses || !PyCallable_Check(args[1])) {
     PyErr_SetString(PyExc_ValueError, "set_fallback(which, callable)");
     return nullptr;
   }
@@ -312,6 +556,13 @@ PyMethodDef g_methods[] = {
     T2FW_METHOD("fused_apply", py_fused_apply, "apply(qkvg, state, n_head) -> (outputs, next_state)"),
     T2FW_METHOD("decode_step", py_decode_step, "decode_step(x, f, query, key, f_key, state_in, state_out, outputs)"),
     T2FW_METHOD("decode_ring", py_decode_ring, "decode_ring(x, f, query, key, f_key, state, outputs) -> bool"),
+    T2FW_METHOD("glr_apply", py_glr_apply, "apply(value, forget, state) -> (outputs, next_state)"),
+    T2FW_METHOD("glr_fused_apply", py_glr_fused_apply, "apply(vg, state) -> (outputs, next_state)"),
+    T2FW_METHOD("rms_apply", py_rms_apply, "apply(x, weight, eps) -> y"),
+    T2FW_METHOD("add_rms_apply", py_add_rms_apply, "apply(x, residual, weight, eps) -> (y, sum)"),
+    T2FW_METHOD("rms_e4m3", py_rms_e4m3, "rms_e4m3(x, residual or None, weight, eps) -> (q, scale[, sum])"),
+    T2FW_METHOD("glr_step", py_glr_step, "glr_step(value, forget, state_in, state_out, outputs)"),
+    T2FW_METHOD("grad_clip", py_grad_clip, "grad_clip(list, max_norm, in_place) -> total or (total, list)"),
     T2FW_METHOD("no_second_derivative", py_no_second_derivative, "no_second_derivative(gradients, tensors) -> gradients"),
     T2FW_METHOD("set_fallback", py_set_fallback, "set_fallback(which, callable)"),
     {nullptr, nullptr, 0, nullptr}};

@@ -3,46 +3,15 @@
 // t2fw/csrc/dfw.cpp:66-69).  This file is only an adapter: it validates tensors, allocates the
 // outputs (and scratch) with the caching allocator, picks the caller's device and current
 // stream, and forwards raw pointers to the C ABI in include/t2fw_b200.h.
-#include <ATen/ATen.h>
-#include <ATen/cuda/CUDAContext.h>
-#include <ATen/cuda/EmptyTensor.h>
-#include <c10/cuda/CUDACachingAllocator.h>
-#include <c10/cuda/CUDAGuard.h>
-#include <torch/library.h>
-
 #include <cstdlib>
 #include <vector>
 
-#include "t2fw_b200.h"
 #include "torch_ops.h"
+#include "torch_util.h"
 
 namespace t2fw_ops {
 
 namespace {
-
-#define T2FW_CHECK_INPUT(x)                                             \
-  TORCH_CHECK((x).device().is_cuda(), #x " must be a CUDA tensor");     \
-  TORCH_CHECK((x).is_contiguous(), #x " must be contiguous")
-
-int dtype_code(const at::Tensor &t) {
-  switch (t.scalar_type()) {
-    case at::kHalf: return T2FW_F16;
-    case at::kBFloat16: return T2FW_BF16;
-    case at::kFloat: return T2FW_F32;
-    case at::kDouble: return T2FW_F64;
-    default: TORCH_CHECK(false, "t2fw: unsupported dtype ", t.scalar_type());
-  }
-  return -1;
-}
-
-void check_status(int rc, const char *what) {
-  TORCH_CHECK(rc == T2FW_OK, what, " failed (status ", rc, "): ", t2fw_last_error());
-}
-
-void check_same(const at::Tensor &a, const at::Tensor &ref, const char *name) {
-  TORCH_CHECK(a.scalar_type() == ref.scalar_type(), name, ": dtype differs from the first tensor's");
-  TORCH_CHECK(a.device() == ref.device(), name, ": device differs from the first tensor's");
-}
 
 int64_t ckpt_interval(int64_t T, int64_t D, int64_t K, int dtype) {
   if (const char *e = std::getenv("T2FW_CKPT_EVERY")) {
@@ -50,19 +19,6 @@ int64_t ckpt_interval(int64_t T, int64_t D, int64_t K, int dtype) {
     if (v > 0) return v;
   }
   return t2fw_lfw_default_ckpt_every(T, D, K, dtype);
-}
-
-// Uninitialised tensors of `like`'s device straight from the caching allocator: a call makes up to seven
-// of them, and each trip through the dispatcher costs about as much host time as a kernel launch.
-at::Tensor new_tensor(at::IntArrayRef sizes, at::ScalarType dtype, const at::Tensor &like) {
-  return at::Tensor(at::detail::empty_cuda(sizes, dtype, like.device(), std::nullopt));
-}
-at::Tensor new_like(const at::Tensor &t) { return new_tensor(t.sizes(), t.scalar_type(), t); }
-
-// Scratch of one call: freed when the call returns, which the caching allocator orders on the stream.
-c10::DataPtr make_scratch(size_t bytes) {
-  if (bytes == 0) return c10::DataPtr();
-  return c10::cuda::CUDACachingAllocator::get()->allocate(bytes);
 }
 
 }  // namespace

@@ -6,6 +6,7 @@ That call allocates its outputs, so the state changes address every step.  The a
 the addresses fixed:
 
   lfw_decode_step(...)   one step into caller-owned `outputs` and `state_out`
+  glr_decode_step(...)   the same for the gated linear recurrence (t2fw_b200/functional_glr.py)
   LFWDecodeLoop          a ring of input slots; one trip round the ring is one launch: a kernel that keeps
                          the state in registers over the ring where it fits (16-bit storage, K = 32, 64
                          or 128), else a CUDA graph of single steps over two alternating state buffers
@@ -24,6 +25,14 @@ def lfw_decode_step(x, f, query, key, f_key, state_in, state_out, outputs):
     `state_out` must be a different buffer from `state_in`."""
     if _ops.decode_step(x, f, query, key, f_key, state_in, state_out, outputs) is NotImplemented:
         torch.ops.lfw.decode_step(x, f, query, key, f_key, state_in, state_out, outputs)
+    return outputs, state_out
+
+
+def glr_decode_step(value, forget, state_in, state_out, outputs):
+    """h' = forget h + value, the gated linear recurrence's step; writes `outputs` [B,1,D] and `state_out` [B,D].
+    `state_out` may be `state_in`: an element is read and written by the same thread."""
+    if _ops.glr_step(value, forget, state_in, state_out, outputs) is NotImplemented:
+        torch.ops.glr.decode_step(value, forget, state_in, state_out, outputs)
     return outputs, state_out
 
 
