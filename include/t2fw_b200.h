@@ -338,7 +338,8 @@ int t2fw_rms_norm_backward(const void *grad_y, const void *grad_sum, const void 
  * c = min(1, max_norm / (total + 1e-6)).  The lists are HOST arrays of device addresses, element counts (positive) and
  * dtypes, which may differ; the tensors are dense.  total is one device number, fp32 or fp64.  out[i] == tensors[i] for
  * all i scales in place (nothing is written where c = 1; the tensors must not overlap), else the outputs overlap no input.
- * Sums are kept in fp64; a total that is infinite or NaN goes into c as it is.
+ * Sums are kept in fp64 (for a total in fp32, the squares of eight neighbouring 16-bit values are added in fp32 first); a
+ * total that is infinite or NaN goes into c as it is.
  */
 size_t t2fw_grad_clip_scratch_bytes(int64_t n_tensors);
 int t2fw_grad_norm(const void *const *tensors, const int64_t *numel, const int *dtype, int64_t n, void *total,

@@ -178,6 +178,8 @@ int lfw_fused_backward(const void *go, const void *gs, const void *qkvg, const v
                        void *d_qkvg, void *ds, int64_t B, int64_t T, int H, int dtype, void *scratch,
                        cudaStream_t st);
 int lfw_chunk_umma_status();
+int lfw_chunk_status_ptr(int **out);      // device address of the status word that a wait which gave up sets
+int lfw_chunk_sm_count(int *out);         // SMs of the current device
 bool lfw_decode_bulk_supported(int64_t B, int64_t D, int64_t K, int dtype);
 int lfw_decode_bulk_forward(const void *x, const void *f, const void *q, const void *k,
                             const void *fk, const void *state, void *out, void *new_state,

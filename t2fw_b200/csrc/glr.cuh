@@ -1,13 +1,17 @@
 // Pieces of the gated linear recurrence's kernels: vectors of a thread's channels, the gate, composition of maps.
 #pragma once
 
+#include <type_traits>
+
+#include "async_copy.cuh"
 #include "common.cuh"
+#include "steps.cuh"
 
 namespace t2fw {
 namespace glr {
 
-// V neighbouring channels as they lie in memory: 16 bytes, or one element.
-template <typename T, int V> struct Raw { using type = uint4; };
+// V neighbouring channels as they lie in memory: 16 bytes, two 16-bit elements, or one element.
+template <typename T, int V> struct Raw { using type = typename std::conditional<V * sizeof(T) == 16, uint4, uint32_t>::type; };
 template <typename T> struct Raw<T, 1> { using type = T; };
 
 template <typename T, int V, typename A>
@@ -53,33 +57,68 @@ __device__ __forceinline__ typename Raw<T, V>::type pack(const A (&v)[V]) {
   return u;
 }
 
-// a = sigmoid(g) and rest = 1 - a, both to full relative precision: from exp(-|g|), which does not overflow.  For 16-bit
-// storage the exponential and the quotient are the fast ones: a few units of 2^-23, where the result is rounded to 2^-9 or
-// 2^-12.  A NaN stays.
+// e = exp(-g), a = sigmoid(g) = 1 / (1 + e) and rest = 1 - a = e a, each to full relative precision.  -g is held at 80 (700):
+// beyond that a is below 2e-35, and e would overflow.  For 16-bit storage the exponential and the reciprocal are the fast ones:
+// some units of 2^-23, where the result is rounded to 2^-9 or 2^-12.  A NaN stays.
 template <bool kFast>
 __device__ __forceinline__ void gate_pair(float g, float &a, float &rest) {
-  const float e = kFast ? __expf(-fabsf(g)) : expf(-fabsf(g));
-  const float hi = kFast ? __fdividef(1.f, 1.f + e) : 1.f / (1.f + e), lo = e * hi;
-  a = g >= 0.f ? hi : lo;
-  rest = g >= 0.f ? lo : hi;
+  float x, e;
+  asm("min.NaN.f32 %0, %1, %2;" : "=f"(x) : "f"(-g), "f"(80.f));
+  if constexpr (kFast) {
+    e = __expf(x);
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(a) : "f"(1.f + e));
+  } else {
+    e = expf(x);
+    a = 1.f / (1.f + e);
+  }
+  rest = e * a;
 }
 template <bool kFast>
 __device__ __forceinline__ void gate_pair(double g, double &a, double &rest) {
-  const double e = exp(-fabs(g)), hi = 1.0 / (1.0 + e), lo = e * hi;
-  a = g >= 0.0 ? hi : lo;
-  rest = g >= 0.0 ? lo : hi;
+  const double e = exp(-g > 700.0 ? 700.0 : -g);
+  a = 1.0 / (1.0 + e);
+  rest = e * a;
 }
 
-// A run of steps acts on the state as h -> P h + L.  A product P that left the range upwards is harmless where the state it
-// meets is exactly zero, and a product that is exactly zero stays so: both are what the steps one by one would give.  (Where a
-// step's own gate is infinite or NaN, L is no finite number either.)
-template <typename A>
-__device__ __forceinline__ A apply(A P, A L, A h) { return h == A(0) ? L : P * h + L; }
-template <typename A>
-__device__ __forceinline__ A product(A first, A then) { return first == A(0) ? A(0) : first * then; }
+// A run of steps acts on the state as c -> P c + S.  A product P that leaves the range upwards is held at the largest finite
+// number, so that a state of zero stays one (P c is 0, not infinity times zero) and a gate of zero ends what was before.
+// Where the steps themselves would meet an infinity or a NaN, S is none either.
+__device__ __forceinline__ float held(float P) {
+  float r;      // |P| or the limit, whichever is less, with P's sign; a NaN stays
+  asm("min.NaN.xorsign.abs.f32 %0, %1, %2;" : "=f"(r) : "f"(P), "f"(3.402823466e38f));
+  return r;
+}
+__device__ __forceinline__ double held(double P) {
+  return P > 1.7976931348623157e308 ? 1.7976931348623157e308 : P < -1.7976931348623157e308 ? -1.7976931348623157e308 : P;
+}
+
+// V products, V sums of products: pairs of fp32 in one instruction.
+template <typename A, int V>
+__device__ __forceinline__ void mul_v(A (&r)[V], const A (&a)[V], const A (&b)[V]) {
+  if constexpr (std::is_same<A, float>::value && V % 2 == 0) {
+#pragma unroll
+    for (int k = 0; k < V; k += 2)
+      steps::unpack2(steps::mul2(steps::pack2(a[k], a[k + 1]), steps::pack2(b[k], b[k + 1])), r[k], r[k + 1]);
+  } else {
+#pragma unroll
+    for (int k = 0; k < V; ++k) r[k] = a[k] * b[k];
+  }
+}
+template <typename A, int V>
+__device__ __forceinline__ void fma_v(A (&r)[V], const A (&a)[V], const A (&b)[V], const A (&c)[V]) {
+  if constexpr (std::is_same<A, float>::value && V % 2 == 0) {
+#pragma unroll
+    for (int k = 0; k < V; k += 2)
+      steps::unpack2(steps::fma2(steps::pack2(a[k], a[k + 1]), steps::pack2(b[k], b[k + 1]), steps::pack2(c[k], c[k + 1])),
+                     r[k], r[k + 1]);
+  } else {
+#pragma unroll
+    for (int k = 0; k < V; ++k) r[k] = a[k] * b[k] + c[k];
+  }
+}
 
 // ---- asynchronous 16-byte copies into shared memory, and a cluster's shared memory --------------------
-__device__ __forceinline__ uint32_t smem_u32(const void *p) { return static_cast<uint32_t>(__cvta_generic_to_shared(p)); }
+using acp::smem_u32;
 __device__ __forceinline__ void copy16(uint32_t dst, const void *src, bool ok) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(ok ? 16 : 0) : "memory");
 }
@@ -92,11 +131,32 @@ __device__ __forceinline__ uint32_t peer_address(uint32_t own, uint32_t rank) {
   asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(own), "r"(rank));
   return r;
 }
-__device__ __forceinline__ void peer_store(uint32_t at, float2 v) {
-  asm volatile("st.shared::cluster.v2.f32 [%0], {%1, %2};" ::"r"(at), "f"(v.x), "f"(v.y) : "memory");
+// Two values into another block's shared memory; their bytes are counted on that block's barrier.
+__device__ __forceinline__ void peer_send(uint32_t at, float2 v, uint32_t bar) {
+  asm volatile("st.async.weak.shared::cluster.mbarrier::complete_tx::bytes.v2.f32 [%0], {%1, %2}, [%3];" ::"r"(at), "f"(v.x),
+               "f"(v.y), "r"(bar) : "memory");
 }
-__device__ __forceinline__ void peer_store(uint32_t at, double2 v) {
-  asm volatile("st.shared::cluster.v2.f64 [%0], {%1, %2};" ::"r"(at), "d"(v.x), "d"(v.y) : "memory");
+__device__ __forceinline__ void peer_send(uint32_t at, double2 v, uint32_t bar) {
+  asm volatile("st.async.weak.shared::cluster.mbarrier::complete_tx::bytes.v2.f64 [%0], {%1, %2}, [%3];" ::"r"(at), "d"(v.x),
+               "d"(v.y), "r"(bar) : "memory");
+}
+// Bounded wait for what the blocks of the cluster send; false if it gave up.
+__device__ __forceinline__ bool peer_wait(uint64_t *bar, uint32_t parity) {
+#pragma unroll 1
+  for (uint32_t i = 0; i < acp::kSpinLimit; ++i) {
+    uint32_t ok;
+    asm volatile(
+        "{\n"
+        ".reg .pred p;\n"
+        "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2, 2000;\n"
+        "selp.u32 %0, 1, 0, p;\n"
+        "}\n"
+        : "=r"(ok)
+        : "r"(smem_u32(bar)), "r"(parity)
+        : "memory");
+    if (ok) return true;
+  }
+  return false;
 }
 // Every thread of every block of the cluster; writes before it are seen behind it.
 __device__ __forceinline__ void cluster_sync() {

@@ -2,16 +2,17 @@
 //
 //   total = sqrt(sum over all tensors and elements of g^2),   c = min(1, max_norm / (total + 1e-6)),   g' = c g
 //
-// Two kinds of launch.  The first leaves one partial sum per block; the second adds them up in each block, in the same order,
-// and scales.  The tensors' addresses and sizes travel as kernel arguments, so a call needs no table in device memory and can be
-// captured.  Work is cut into pieces of 16 KB; a block takes consecutive ones.
-#include "common.cuh"
+// Two launches.  The first leaves one partial sum per block; the second adds them up in each block, in the same order, and
+// scales.  The tensors' addresses and sizes travel as kernel arguments, so a call needs no table in device memory and can be
+// captured.  Work is cut into pieces of 32 KB that begin at 16-byte boundaries, whatever the tensor's own address; a block takes
+// consecutive ones.  Bound by memory: the sums take one conversion to fp64 per vector of 16-bit values, per value in fp32.
+#include "glr.cuh"
 
 namespace t2fw {
 
 namespace {
 
-constexpr int kTable = 512, kThreads = 256, kPieceBytes = 16384, kMaxBlocks = 592;
+constexpr int kTable = 512, kThreads = 256, kPieceBytes = 32768, kVectors = kPieceBytes / (16 * kThreads), kMaxBlocks = 592;
 
 struct Entry {
   const void *in;
@@ -49,25 +50,116 @@ __device__ __forceinline__ int find(const Table<N> &t, uint32_t p) {
   return lo;
 }
 
+// Sum of squares of a vector, in fp64.  For a total in fp32, the eight squares of 16-bit values are added in fp32 first (off by
+// 2^-22 at most, each vector another way); where the sum is not well inside fp32's range, which bf16 can leave, in fp64 too.
 template <typename T>
-__device__ __forceinline__ double squares(const T *in, int64_t from, int64_t to) {
-  double s = 0;
-  for (int64_t i = from + threadIdx.x; i < to; i += kThreads) {
-    const double v = (double)Elem<T>::ld(in + i);
-    s += v * v;
+__device__ __forceinline__ double squares(const uint4 &u, bool exact) {
+  if constexpr (sizeof(T) == 2) {
+    float v[8], q = 0.f;
+    glr::unpack<T, 8>(u, v);
+#pragma unroll
+    for (int k = 0; k < 8; ++k) q += v[k] * v[k];
+    if (!exact && q > 0x1p-90f && q < 0x1p120f) return (double)q;
+    if (((u.x | u.y | u.z | u.w) & 0x7fff7fffu) == 0) return 0.0;
+    double s = 0;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) s += (double)v[k] * (double)v[k];
+    return s;
+  } else {
+    constexpr int V = 16 / sizeof(T);
+    const T *p = reinterpret_cast<const T *>(&u);
+    double s = 0;
+#pragma unroll
+    for (int k = 0; k < V; ++k) s += (double)p[k] * (double)p[k];
+    return s;
   }
+}
+
+// Where a piece lies: `at` its first byte and [from, to) the tensor's own bytes, all counted from the 16-byte boundary at or
+// below the tensor's address.
+struct Piece {
+  const unsigned char *in;
+  int64_t at, from, to;
+};
+template <int N>
+__device__ __forceinline__ Piece piece_of(const Table<N> &t, int k, uint32_t p, int bytes) {
+  const uintptr_t a = reinterpret_cast<uintptr_t>(t.e[k].in);
+  Piece r;
+  r.from = (int64_t)(a & 15);
+  r.in = static_cast<const unsigned char *>(t.e[k].in) - r.from;
+  r.to = r.from + t.e[k].n * bytes;
+  r.at = (int64_t)(p - t.first[k]) * kPieceBytes;
+  return r;
+}
+
+template <typename T>
+__device__ __forceinline__ double piece_squares(const Piece &r, bool exact) {
+  double s = 0;
+  uint4 u[kVectors];
+#pragma unroll
+  for (int j = 0; j < kVectors; ++j) {
+    const int64_t o = r.at + (int64_t)(threadIdx.x + j * kThreads) * 16;
+    u[j] = make_uint4(0, 0, 0, 0);
+    if (o >= r.from && o + 16 <= r.to) {
+      u[j] = *reinterpret_cast<const uint4 *>(r.in + o);
+    } else if (o + 16 > r.from && o < r.to) {      // the tensor's first or last vector
+      T *e = reinterpret_cast<T *>(&u[j]);
+#pragma unroll
+      for (int k = 0; k < 16 / (int)sizeof(T); ++k) {
+        const int64_t q = o + k * (int64_t)sizeof(T);
+        if (q >= r.from && q < r.to) e[k] = *reinterpret_cast<const T *>(r.in + q);
+      }
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < kVectors; ++j) s += squares<T>(u[j], exact);
   return s;
 }
 
+// `out` is the address that corresponds to r.in; whole vectors where it is aligned too.
 template <typename T, typename C>
-__device__ __forceinline__ void scale(const T *in, T *out, int64_t from, int64_t to, C c) {
+__device__ __forceinline__ void piece_scale(const Piece &r, unsigned char *out, C c) {
   using A = typename Elem<T>::acc;
-  for (int64_t i = from + threadIdx.x; i < to; i += kThreads) Elem<T>::st(out + i, (A)Elem<T>::ld(in + i) * (A)c);
+  constexpr int V = 16 / sizeof(T), kHalf = kVectors / 2;
+  const bool aligned = (reinterpret_cast<uintptr_t>(out) & 15) == 0;
+  if (aligned) {
+#pragma unroll 1
+    for (int h = 0; h < 2; ++h) {
+      uint4 u[kHalf];
+      const int64_t o0 = r.at + (int64_t)(threadIdx.x + h * kHalf * kThreads) * 16;
+#pragma unroll
+      for (int j = 0; j < kHalf; ++j) {
+        const int64_t o = o0 + j * kThreads * 16;
+        if (o >= r.from && o + 16 <= r.to) u[j] = __ldcs(reinterpret_cast<const uint4 *>(r.in + o));
+      }
+#pragma unroll
+      for (int j = 0; j < kHalf; ++j) {
+        const int64_t o = o0 + j * kThreads * 16;
+        if (o >= r.from && o + 16 <= r.to) {
+          A v[V];
+          glr::unpack<T, V>(u[j], v);
+#pragma unroll
+          for (int k = 0; k < V; ++k) v[k] *= (A)c;
+          __stcs(reinterpret_cast<uint4 *>(out + o), glr::pack<T, V>(v));
+        }
+      }
+    }
+    if (r.at >= r.from && r.at + kPieceBytes <= r.to) return;
+  }
+  // the tensor's first and last vector, and outputs at another offset within 16 bytes: element by element
+#pragma unroll 1
+  for (int j = 0; j < kVectors; ++j) {
+    const int64_t o = r.at + (int64_t)(threadIdx.x + j * kThreads) * 16;
+    if (aligned && o >= r.from && o + 16 <= r.to) continue;
+#pragma unroll 1
+    for (int64_t q = o > r.from ? o : r.from; q < o + 16 && q < r.to; q += (int64_t)sizeof(T))
+      Elem<T>::st(reinterpret_cast<T *>(out + q), (A)Elem<T>::ld(reinterpret_cast<const T *>(r.in + q)) * (A)c);
+  }
 }
 
 template <int N>
-__global__ void __launch_bounds__(kThreads)
-grad_norm_kernel(const __grid_constant__ Table<N> t, double *__restrict__ part) {
+__global__ void __launch_bounds__(kThreads, 4)
+grad_norm_kernel(const __grid_constant__ Table<N> t, double *__restrict__ part, bool exact) {
   __shared__ double red[kThreads / 32];
   dependency_wait();
   const uint32_t pieces = t.first[t.count];
@@ -77,15 +169,11 @@ grad_norm_kernel(const __grid_constant__ Table<N> t, double *__restrict__ part) 
   double s = 0;
   for (uint32_t p = p0; p < p1; ++p) {
     while (p >= t.first[k + 1]) ++k;
-    const int bytes = t.type[k] == T2FW_F64 ? 8 : t.type[k] == T2FW_F32 ? 4 : 2;
-    const int64_t per = kPieceBytes / bytes, from = (int64_t)(p - t.first[k]) * per;
-    const int64_t to = from + per < t.e[k].n ? from + per : t.e[k].n;
-    const void *in = t.e[k].in;
     switch (t.type[k]) {
-      case T2FW_F16: s += squares(static_cast<const __half *>(in), from, to); break;
-      case T2FW_BF16: s += squares(static_cast<const __nv_bfloat16 *>(in), from, to); break;
-      case T2FW_F32: s += squares(static_cast<const float *>(in), from, to); break;
-      default: s += squares(static_cast<const double *>(in), from, to); break;
+      case T2FW_F16: s += piece_squares<__half>(piece_of(t, k, p, 2), exact); break;
+      case T2FW_BF16: s += piece_squares<__nv_bfloat16>(piece_of(t, k, p, 2), exact); break;
+      case T2FW_F32: s += piece_squares<float>(piece_of(t, k, p, 4), exact); break;
+      default: s += piece_squares<double>(piece_of(t, k, p, 8), exact); break;
     }
   }
   s = block_sum(s, red);
@@ -94,7 +182,7 @@ grad_norm_kernel(const __grid_constant__ Table<N> t, double *__restrict__ part) 
 
 // max_norm < 0: only the norm is wanted.
 template <int N, typename C>
-__global__ void __launch_bounds__(kThreads)
+__global__ void __launch_bounds__(kThreads, 4)
 grad_scale_kernel(const __grid_constant__ Table<N> t, const double *__restrict__ part, int n_part, double max_norm,
                   C *__restrict__ total, bool in_place) {
   __shared__ double red[kThreads / 32];
@@ -114,16 +202,12 @@ grad_scale_kernel(const __grid_constant__ Table<N> t, const double *__restrict__
   int k = find(t, p1 - 1);
   for (uint32_t p = p1; p-- > p0;) {      // backwards: what the first launch read last is still in L2
     while (p < t.first[k]) --k;
-    const int bytes = t.type[k] == T2FW_F64 ? 8 : t.type[k] == T2FW_F32 ? 4 : 2;
-    const int64_t per = kPieceBytes / bytes, from = (int64_t)(p - t.first[k]) * per;
-    const int64_t to = from + per < t.e[k].n ? from + per : t.e[k].n;
-    const void *in = t.e[k].in;
-    void *out = t.e[k].out;
+    unsigned char *out = static_cast<unsigned char *>(t.e[k].out) - (reinterpret_cast<uintptr_t>(t.e[k].in) & 15);
     switch (t.type[k]) {
-      case T2FW_F16: scale(static_cast<const __half *>(in), static_cast<__half *>(out), from, to, c); break;
-      case T2FW_BF16: scale(static_cast<const __nv_bfloat16 *>(in), static_cast<__nv_bfloat16 *>(out), from, to, c); break;
-      case T2FW_F32: scale(static_cast<const float *>(in), static_cast<float *>(out), from, to, c); break;
-      default: scale(static_cast<const double *>(in), static_cast<double *>(out), from, to, c); break;
+      case T2FW_F16: piece_scale<__half>(piece_of(t, k, p, 2), out, c); break;
+      case T2FW_BF16: piece_scale<__nv_bfloat16>(piece_of(t, k, p, 2), out, c); break;
+      case T2FW_F32: piece_scale<float>(piece_of(t, k, p, 4), out, c); break;
+      default: piece_scale<double>(piece_of(t, k, p, 8), out, c); break;
     }
   }
 }
@@ -136,7 +220,8 @@ int fill(Table<N> &t, const void *const *in, void *const *out, const int64_t *nu
   for (; k < N && at + k < n; ++k) {
     t.e[k] = {in[at + k], out != nullptr ? out[at + k] : nullptr, numel[at + k]};
     t.type[k] = (uint8_t)dtype[at + k];
-    t.first[k + 1] = t.first[k] + (uint32_t)ceil_div64(numel[at + k] * (int64_t)dtype_size(dtype[at + k]), kPieceBytes);
+    const int64_t lead = (int64_t)(reinterpret_cast<uintptr_t>(in[at + k]) & 15);
+    t.first[k + 1] = t.first[k] + (uint32_t)ceil_div64(lead + numel[at + k] * (int64_t)dtype_size(dtype[at + k]), kPieceBytes);
   }
   t.count = k;
   return k;
@@ -156,7 +241,8 @@ int run(const void *const *in, void *const *out, const int64_t *numel, const int
   for (int at = 0; at < n;) {
     at += fill(t, in, out, numel, dtype, at, n);
     const unsigned g = blocks_of(t);
-    T2FW_CHECK_CUDA(launch_dependent(grad_norm_kernel<N>, dim3(g), dim3(kThreads), 0, st, t, part + n_part));
+    T2FW_CHECK_CUDA(launch_dependent(grad_norm_kernel<N>, dim3(g), dim3(kThreads), 0, st, t, part + n_part,
+                                     sizeof(C) == 8));
     T2FW_CHECK_LAUNCH(1);
     n_part += (int)g;
   }

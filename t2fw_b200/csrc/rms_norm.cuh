@@ -1,0 +1,541 @@
+// Root-mean-square norm over rows of D, with or without the addition of a residual, and its gradients:
+//
+//   s = x + residual,  rstd = 1 / sqrt(mean(s^2) + eps),  y = s rstd w
+//   g = w dy:   d_s = rstd (g - s rstd^2 mean(g s)) + (gradient of s from its other use) ,   d_w = sum over rows of dy s rstd
+//
+// x and the residual share the gradient d_s.  The 8-bit form leaves q = e4m3(y / scale) with scale = max|y| / 448 per row;
+// max|y| = rstd max|s w|, so both sums of a row are formed at once, and so are both of the gradients' (s^2 and g s).
+#pragma once
+
+#include <cuda_fp8.h>
+
+#include <initializer_list>
+
+#include "glr.cuh"
+
+namespace t2fw {
+namespace rms {
+
+using glr::Raw;
+using glr::pack;
+using glr::unpack;
+
+constexpr float kE4m3Max = 448.f, kMinScale = 1e-30f;
+
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ float inv_sqrt(float v) { return 1.f / sqrtf(v); }
+__device__ __forceinline__ double inv_sqrt(double v) { return 1.0 / sqrt(v); }
+
+// Two reductions over the GS threads of a row at once, the results in each of them; kMax: the second is a maximum.  `red`
+// alternates between two halves, so a block needs one barrier per row.
+template <int GS, bool kMax, typename A>
+__device__ __forceinline__ void row_reduce(A &a, A &b, A (*red)[2]) {
+#pragma unroll
+  for (int o = (GS < 32 ? GS : 32) / 2; o > 0; o >>= 1) {
+    a += __shfl_xor_sync(0xffffffffu, a, o);
+    const A t = __shfl_xor_sync(0xffffffffu, b, o);
+    if constexpr (kMax) b = max_nan(b, t);
+    else b += t;
+  }
+  if constexpr (GS > 32) {
+    constexpr int W = GS / 32;
+    if ((threadIdx.x & 31) == 0) {
+      red[threadIdx.x >> 5][0] = a;
+      red[threadIdx.x >> 5][1] = b;
+    }
+    __syncthreads();
+    a = red[0][0];
+    b = red[0][1];
+#pragma unroll
+    for (int i = 1; i < W; ++i) {
+      a += red[i][0];
+      if constexpr (kMax) b = max_nan(b, red[i][1]);
+      else b += red[i][1];
+    }
+  }
+}
+
+// V values as e4m3, one behind the other.
+template <int V> struct Raw8 { using type = uint2; };
+template <> struct Raw8<4> { using type = uint32_t; };
+template <> struct Raw8<1> { using type = __nv_fp8_storage_t; };
+template <int V>
+__device__ __forceinline__ typename Raw8<V>::type pack8(const float (&v)[V]) {
+  if constexpr (V == 1) {
+    return __nv_cvt_float_to_fp8(v[0], __NV_SATFINITE, __NV_E4M3);
+  } else {
+    typename Raw8<V>::type u;
+    __nv_fp8x2_storage_t *p = reinterpret_cast<__nv_fp8x2_storage_t *>(&u);
+#pragma unroll
+    for (int i = 0; i < V / 2; ++i)
+      p[i] = __nv_cvt_float2_to_fp8x2(make_float2(v[2 * i], v[2 * i + 1]), __NV_SATFINITE, __NV_E4M3);
+    return u;
+  }
+}
+
+template <typename T>
+struct FwdArgs {
+  const T *x, *r, *w;      // r: null without a residual
+  T *y, *sum;
+  void *q;
+  float *scale;
+  int64_t rows, D;
+  double eps;
+};
+template <typename T>
+struct BwdArgs {
+  const T *dy, *dsum, *s, *w;      // dsum: null for zero
+  T *ds;
+  typename Elem<T>::acc *part;
+  int64_t rows, D;
+  double eps;
+};
+
+template <int GS> constexpr int block_of() { return GS <= 32 ? 256 : GS; }
+
+// sums += a b, element by element; pairs of fp32 in one instruction
+template <typename A, int V>
+__device__ __forceinline__ void add_products(A (&sums)[2], const A (&a)[V], const A (&b)[V]) {
+  if constexpr (V == 1) {
+    sums[0] += a[0] * b[0];
+  } else {
+#pragma unroll
+    for (int k = 0; k < V; k += 2) {
+      const A x[2] = {a[k], a[k + 1]}, y[2] = {b[k], b[k + 1]};
+      glr::fma_v(sums, x, y, sums);
+    }
+  }
+}
+
+// A row on GS threads, NV vectors of V elements each, in registers; the next row's values are on their way while a row is
+// reduced.  GS <= 32: several rows in a block, a warp or a part of one each.
+template <typename T, int V, int NV, int GS, bool k8>
+__global__ void __launch_bounds__(block_of<GS>())
+rms_fwd_kernel(const FwdArgs<T> p) {
+  using A = typename Elem<T>::acc;
+  using R = typename Raw<T, V>::type;
+  constexpr int kRows = block_of<GS>() / GS;
+  __shared__ A red[2][GS > 32 ? GS / 32 : 1][2];
+  dependency_wait();
+  const int tid = threadIdx.x % GS;
+  const int64_t step = (int64_t)gridDim.x * kRows;
+  const A inv_d = A(1) / A(p.D), eps = (A)p.eps;
+  const bool add = p.r != nullptr;
+  R x[NV], r[NV], w[NV];
+  bool on[NV];
+#pragma unroll
+  for (int i = 0; i < NV; ++i) on[i] = (int64_t)(tid + i * GS) * V < p.D;
+  auto load = [&](int64_t row) {
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int64_t at = row * p.D + (int64_t)(tid + i * GS) * V;
+      x[i] = R{};
+      if (on[i]) x[i] = *reinterpret_cast<const R *>(p.x + at);
+      if (add) {
+        r[i] = R{};
+        if (on[i]) r[i] = *reinterpret_cast<const R *>(p.r + at);
+      }
+    }
+  };
+  // all rows of a block take the same number of rounds, so that whole warps meet in the reductions
+  const int64_t first = (int64_t)blockIdx.x * kRows;
+  int64_t row = first + threadIdx.x / GS;
+  bool valid = row < p.rows;
+#pragma unroll
+  for (int i = 0; i < NV; ++i) x[i] = r[i] = w[i] = R{};
+  if (valid) load(row);
+#pragma unroll
+  for (int i = 0; i < NV; ++i)
+    if (on[i]) w[i] = *reinterpret_cast<const R *>(p.w + (tid + i * GS) * V);
+  for (int64_t base = first, half = 0; base < p.rows; base += step, row += step, half ^= 1) {
+    A s[NV][V], sums[2] = {A(0), A(0)}, top = A(0);
+    valid = row < p.rows;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      unpack<T, V>(x[i], s[i]);
+      if (add) {
+        A t[V];
+        unpack<T, V>(r[i], t);
+#pragma unroll
+        for (int k = 0; k < V; ++k) s[i][k] += t[k];
+        if (on[i] && valid) *reinterpret_cast<R *>(p.sum + row * p.D + (int64_t)(tid + i * GS) * V) = pack<T, V>(s[i]);
+      }
+    }
+    if (row + step < p.rows) load(row + step);
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      A wv[V];
+      if constexpr (k8) unpack<T, V>(w[i], wv);
+      add_products(sums, s[i], s[i]);
+      if constexpr (k8) {
+        glr::mul_v(wv, wv, s[i]);
+#pragma unroll
+        for (int k = 0; k < V; ++k) top = max_nan(top, fabsf(wv[k]));
+      }
+    }
+    A ss = sums[0] + sums[1];
+    row_reduce<GS, k8>(ss, top, red[half]);
+    const A rstd = inv_sqrt(ss * inv_d + eps);
+    A f = rstd;
+    if constexpr (k8) {
+      const float scale = max_nan(top * rstd / kE4m3Max, kMinScale);
+      if (tid == 0 && valid) p.scale[row] = scale;
+      f = rstd / scale;
+    }
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      A wv[V];
+      unpack<T, V>(w[i], wv);
+      A fv[V];
+#pragma unroll
+      for (int k = 0; k < V; ++k) fv[k] = f;
+      glr::mul_v(s[i], s[i], fv);
+      glr::mul_v(s[i], s[i], wv);
+      const int64_t at = row * p.D + (int64_t)(tid + i * GS) * V;
+      if (on[i] && valid) {
+        if constexpr (k8) *reinterpret_cast<typename Raw8<V>::type *>(static_cast<unsigned char *>(p.q) + at) = pack8<V>(s[i]);
+        else *reinterpret_cast<R *>(p.y + at) = pack<T, V>(s[i]);
+      }
+    }
+  }
+}
+
+// The same for the gradients.  A thread sums the weight gradient of its columns over its rows in registers; a block leaves one
+// line of `part`, and rms_dw_kernel adds the lines up, always in the same order.  Rows on a warp or less are not fetched ahead:
+// 16 warps to an SM with a row each keep more in flight than 8 with two (the registers would not hold more).
+template <typename T, int V, int NV, int GS>
+__global__ void __launch_bounds__(block_of<GS>(), GS >= 512 ? 1 : GS == 128 ? 4 : 2)
+rms_bwd_kernel(const BwdArgs<T> p) {
+  using A = typename Elem<T>::acc;
+  using R = typename Raw<T, V>::type;
+  constexpr int kRows = block_of<GS>() / GS, kCols = NV * GS * V;
+  constexpr bool kAhead = GS > 32, kShared = GS <= 32 && NV > 2;      // where registers are short the weights lie in shared memory
+  __shared__ A red[2][GS > 32 ? GS / 32 : 1][2];
+  __shared__ R s_w[kShared ? NV * GS : 1];
+  __shared__ A lines[kRows > 1 ? kRows / 2 : 1][kRows > 1 ? kCols : 1];
+  dependency_wait();
+  const int tid = threadIdx.x % GS, group = threadIdx.x / GS;
+  const int64_t step = (int64_t)gridDim.x * kRows;
+  const A inv_d = A(1) / A(p.D), eps = (A)p.eps;
+  R dy[NV], s[NV], w[kShared ? 1 : NV];
+  bool on[NV];
+  A dw[NV][V];
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    on[i] = (int64_t)(tid + i * GS) * V < p.D;
+    dy[i] = s[i] = R{};
+#pragma unroll
+    for (int k = 0; k < V; ++k) dw[i][k] = A(0);
+  }
+  auto load = [&](int64_t row) {
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int64_t at = row * p.D + (int64_t)(tid + i * GS) * V;
+      if (on[i]) {
+        dy[i] = *reinterpret_cast<const R *>(p.dy + at);
+        s[i] = *reinterpret_cast<const R *>(p.s + at);
+      }
+    }
+  };
+  const int64_t first = (int64_t)blockIdx.x * kRows;
+  int64_t row = first + group;
+  if (kAhead && row < p.rows) load(row);
+  if constexpr (kShared) {
+    for (int i = threadIdx.x; i < NV * GS; i += block_of<GS>())
+      s_w[i] = (int64_t)i * V < p.D ? *reinterpret_cast<const R *>(p.w + i * V) : R{};
+    __syncthreads();
+  } else {
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      w[i] = R{};
+      if (on[i]) w[i] = *reinterpret_cast<const R *>(p.w + (tid + i * GS) * V);
+    }
+  }
+  auto weight = [&](int i, A (&v)[V]) {
+    if constexpr (kShared) unpack<T, V>(s_w[tid + i * GS], v);
+    else unpack<T, V>(w[i], v);
+  };
+  for (int64_t base = first, half = 0; base < p.rows; base += step, row += step, half ^= 1) {
+    const bool valid = row < p.rows;
+    if (!kAhead && valid) load(row);
+    R up[NV], cdy[NV], cs[NV];
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      if (p.dsum != nullptr && on[i] && valid)
+        up[i] = *reinterpret_cast<const R *>(p.dsum + row * p.D + (int64_t)(tid + i * GS) * V);
+      cdy[i] = dy[i], cs[i] = s[i];
+    }
+    if (kAhead && row + step < p.rows) load(row + step);
+    A s2[2] = {A(0), A(0)}, g2[2] = {A(0), A(0)};
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      A sv[V], g[V], wv[V];
+      unpack<T, V>(cs[i], sv);
+      unpack<T, V>(cdy[i], g);
+      weight(i, wv);
+      add_products(s2, sv, sv);
+      glr::mul_v(g, g, wv);
+      add_products(g2, g, sv);
+    }
+    A ss = s2[0] + s2[1], gs = g2[0] + g2[1];
+    row_reduce<GS, false>(ss, gs, red[half]);
+    const A rstd = inv_sqrt(ss * inv_d + eps), m = gs * inv_d * rstd * rstd * rstd;
+    if (valid) {
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+        A sv[V], g[V], wv[V], v[V], k1[V], k2[V];
+        unpack<T, V>(cs[i], sv);
+        unpack<T, V>(cdy[i], g);
+        weight(i, wv);
+#pragma unroll
+        for (int k = 0; k < V; ++k) k1[k] = rstd, k2[k] = -m;
+        glr::mul_v(g, g, k1);              // rstd dy
+        glr::fma_v(dw[i], g, sv, dw[i]);
+        glr::mul_v(v, sv, k2);
+        glr::fma_v(v, g, wv, v);
+        if (p.dsum != nullptr) {
+          A u[V];
+          unpack<T, V>(up[i], u);
+#pragma unroll
+          for (int k = 0; k < V; ++k) v[k] += u[k];
+        }
+        if (on[i]) *reinterpret_cast<R *>(p.ds + row * p.D + (int64_t)(tid + i * GS) * V) = pack<T, V>(v);
+      }
+    }
+  }
+  // rows of a block: halve their number until one line is left
+#pragma unroll
+  for (int n = kRows / 2; n > 0; n >>= 1) {
+    __syncthreads();
+    if (group >= n && group < 2 * n) {
+#pragma unroll
+      for (int i = 0; i < NV; ++i)
+#pragma unroll
+        for (int k = 0; k < V; ++k) lines[group - n][(i * V + k) * GS + tid] = dw[i][k];
+    }
+    __syncthreads();
+    if (group < n) {
+#pragma unroll
+      for (int i = 0; i < NV; ++i)
+#pragma unroll
+        for (int k = 0; k < V; ++k) dw[i][k] += lines[group][(i * V + k) * GS + tid];
+    }
+  }
+  if (group == 0) {
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+      if (on[i]) {
+        A *to = p.part + (int64_t)blockIdx.x * p.D + (tid + i * GS) * V;
+#pragma unroll
+        for (int k = 0; k < V; ++k) to[k] = dw[i][k];
+      }
+  }
+}
+
+// 32 columns of the lines that the blocks left, each warp every 32nd line.
+template <typename T>
+__global__ void __launch_bounds__(1024)
+rms_dw_kernel(const typename Elem<T>::acc *__restrict__ part, T *__restrict__ dw, int n, int64_t D) {
+  using A = typename Elem<T>::acc;
+  __shared__ A sums[32][33];
+  dependency_wait();
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int64_t d = (int64_t)blockIdx.x * 32 + lane;
+  A v = A(0);
+  if (d < D) {
+#pragma unroll 8
+    for (int i = warp; i < n; i += 32) v += part[(int64_t)i * D + d];
+  }
+  sums[warp][lane] = v;
+  __syncthreads();
+  v = warp_sum(sums[lane][warp]);      // a warp per column now
+  const int64_t c = (int64_t)blockIdx.x * 32 + warp;
+  if (lane == 0 && c < D) Elem<T>::st(dw + c, v);
+}
+
+// ---- rows that no registers hold: a block per row, read again for each use ------------------------------
+template <typename T, bool k8>
+__global__ void __launch_bounds__(512)
+rms_fwd_long_kernel(const FwdArgs<T> p) {
+  using A = typename Elem<T>::acc;
+  __shared__ A red[16][2];
+  dependency_wait();
+  const int64_t base = (int64_t)blockIdx.x * p.D;
+  A ss = A(0), top = A(0);
+  for (int64_t d = threadIdx.x; d < p.D; d += 512) {
+    A s = Elem<T>::ld(p.x + base + d);
+    if (p.r != nullptr) {
+      s += (A)Elem<T>::ld(p.r + base + d);
+      Elem<T>::st(p.sum + base + d, s);
+    }
+    ss += s * s;
+    if constexpr (k8) top = max_nan(top, fabsf(s * (A)Elem<T>::ld(p.w + d)));
+  }
+  row_reduce<512, k8>(ss, top, red);
+  const A rstd = inv_sqrt(ss / A(p.D) + (A)p.eps);
+  A f = rstd;
+  if constexpr (k8) {
+    const float scale = max_nan(top * rstd / kE4m3Max, kMinScale);
+    if (threadIdx.x == 0) p.scale[blockIdx.x] = scale;
+    f = rstd / scale;
+  }
+  for (int64_t d = threadIdx.x; d < p.D; d += 512) {
+    A s = Elem<T>::ld(p.x + base + d);
+    if (p.r != nullptr) s += (A)Elem<T>::ld(p.r + base + d);
+    const A v[1] = {s * f * (A)Elem<T>::ld(p.w + d)};
+    if constexpr (k8) static_cast<__nv_fp8_storage_t *>(p.q)[base + d] = pack8<1>(v);
+    else Elem<T>::st(p.y + base + d, v[0]);
+  }
+}
+
+// Blocks walk rows; the weight gradient of a block's rows is summed in its own line of `part`.
+template <typename T>
+__global__ void __launch_bounds__(512)
+rms_bwd_long_kernel(const BwdArgs<T> p) {
+  using A = typename Elem<T>::acc;
+  __shared__ A red[2][16][2];
+  dependency_wait();
+  A *const mine = p.part + (int64_t)blockIdx.x * p.D;
+  bool first = true;
+  int half = 0;
+  for (int64_t row = blockIdx.x; row < p.rows; row += gridDim.x, half ^= 1) {
+    const int64_t base = row * p.D;
+    A ss = A(0), gs = A(0);
+    for (int64_t d = threadIdx.x; d < p.D; d += 512) {
+      const A sv = Elem<T>::ld(p.s + base + d);
+      ss += sv * sv;
+      gs += (A)Elem<T>::ld(p.dy + base + d) * (A)Elem<T>::ld(p.w + d) * sv;
+    }
+    row_reduce<512, false>(ss, gs, red[half]);
+    const A rstd = inv_sqrt(ss / A(p.D) + (A)p.eps), m = gs / A(p.D) * rstd * rstd;
+    for (int64_t d = threadIdx.x; d < p.D; d += 512) {
+      const A sv = Elem<T>::ld(p.s + base + d), g = Elem<T>::ld(p.dy + base + d);
+      A v = rstd * ((A)Elem<T>::ld(p.w + d) * g - sv * m);
+      if (p.dsum != nullptr) v += (A)Elem<T>::ld(p.dsum + base + d);
+      Elem<T>::st(p.ds + base + d, v);
+      mine[d] = (first ? A(0) : mine[d]) + g * sv * rstd;
+    }
+    first = false;
+  }
+}
+
+// ---- launches ---------------------------------------------------------------------------------------
+// Blocks per SM that the launches below ask for: as many as keep some 100 KB of loads in flight.
+template <int GS> constexpr int blocks_per_sm() { return GS <= 32 ? 4 : GS == 128 ? 8 : GS == 256 ? 4 : 2; }
+
+template <int GS>
+inline int64_t grid_of(int64_t rows, int sms, int per_sm) {
+  const int64_t need = ceil_div64(rows, block_of<GS>() / GS), most = (int64_t)sms * per_sm;
+  return need < most ? need : most;
+}
+
+constexpr int64_t kMostParts = 1024;      // lines of the weight gradient's partial sums; blocks of the backward launches
+inline int64_t capped(int64_t n) { return n < kMostParts ? n : kMostParts; }
+
+template <typename T, int V, int NV, int GS, bool k8>
+int launch_fwd_as(const FwdArgs<T> &p, int sms, cudaStream_t st) {
+  T2FW_CHECK_CUDA(launch_dependent(rms_fwd_kernel<T, V, NV, GS, k8>,
+                                   dim3((unsigned)grid_of<GS>(p.rows, sms, blocks_per_sm<GS>())), dim3(block_of<GS>()), 0, st, p));
+  T2FW_CHECK_LAUNCH(1);
+  return T2FW_OK;
+}
+template <typename T, int V, int NV, int GS>
+int launch_bwd_as(const BwdArgs<T> &p, int sms, int64_t *parts, cudaStream_t st) {
+  *parts = capped(grid_of<GS>(p.rows, sms, blocks_per_sm<GS>() / 2));
+  T2FW_CHECK_CUDA(launch_dependent(rms_bwd_kernel<T, V, NV, GS>, dim3((unsigned)*parts), dim3(block_of<GS>()), 0, st, p));
+  T2FW_CHECK_LAUNCH(1);
+  return T2FW_OK;
+}
+
+// A row on as few threads as hold it: a part of a warp, a warp, four, eight or sixteen.
+template <typename T, int V, bool k8>
+int launch_fwd_v(const FwdArgs<T> &p, int sms, cudaStream_t st) {
+  const int64_t n = ceil_div64(p.D, V);
+  constexpr int M = V == 1 ? 2 : 1;      // single elements: twice as many per thread
+  if (n <= 8 * M) return launch_fwd_as<T, V, 1 * M, 8, k8>(p, sms, st);
+  if (n <= 16 * M) return launch_fwd_as<T, V, 1 * M, 16, k8>(p, sms, st);
+  if (n <= 32 * M) return launch_fwd_as<T, V, 1 * M, 32, k8>(p, sms, st);
+  if (n <= 64 * M) return launch_fwd_as<T, V, 2 * M, 32, k8>(p, sms, st);
+  if (n <= 96 * M) return launch_fwd_as<T, V, 3 * M, 32, k8>(p, sms, st);
+  if (n <= 128 * M) return launch_fwd_as<T, V, 4 * M, 32, k8>(p, sms, st);
+  if (n <= 256 * M) return launch_fwd_as<T, V, 2 * M, 128, k8>(p, sms, st);
+  if (n <= 512 * M) return launch_fwd_as<T, V, 2 * M, 256, k8>(p, sms, st);
+  if (n <= 1024 * M) return launch_fwd_as<T, V, 2 * M, 512, k8>(p, sms, st);
+  if (n <= 2048 * M) return launch_fwd_as<T, V, 4 * M, 512, k8>(p, sms, st);
+  T2FW_CHECK_CUDA(launch_dependent(rms_fwd_long_kernel<T, k8>, dim3((unsigned)p.rows), dim3(512), 0, st, p));
+  T2FW_CHECK_LAUNCH(1);
+  return T2FW_OK;
+}
+template <typename T, int V>
+int launch_bwd_v(const BwdArgs<T> &p, int sms, int64_t *parts, cudaStream_t st) {
+  const int64_t n = ceil_div64(p.D, V);
+  constexpr int M = V == 1 ? 2 : 1;
+  if (n <= 8 * M) return launch_bwd_as<T, V, 1 * M, 8>(p, sms, parts, st);
+  if (n <= 16 * M) return launch_bwd_as<T, V, 1 * M, 16>(p, sms, parts, st);
+  if (n <= 32 * M) return launch_bwd_as<T, V, 1 * M, 32>(p, sms, parts, st);
+  if (n <= 64 * M) return launch_bwd_as<T, V, 2 * M, 32>(p, sms, parts, st);
+  if (n <= 128 * M) return launch_bwd_as<T, V, 1 * M, 128>(p, sms, parts, st);
+  if (n <= 256 * M) return launch_bwd_as<T, V, 2 * M, 128>(p, sms, parts, st);
+  if (n <= 512 * M) return launch_bwd_as<T, V, 2 * M, 256>(p, sms, parts, st);
+  if (n <= 1024 * M) return launch_bwd_as<T, V, 2 * M, 512>(p, sms, parts, st);
+  if constexpr (V < 8)      // with eight values to a vector a thread's registers do not hold them
+    if (n <= 2048 * M) return launch_bwd_as<T, V, 4 * M, 512>(p, sms, parts, st);
+  *parts = capped(p.rows < 2 * sms ? p.rows : 2 * sms);
+  T2FW_CHECK_CUDA(launch_dependent(rms_bwd_long_kernel<T>, dim3((unsigned)*parts), dim3(512), 0, st, p));
+  T2FW_CHECK_LAUNCH(1);
+  return T2FW_OK;
+}
+
+inline bool aligned(std::initializer_list<const void *> ps) {
+  uintptr_t low = 0;
+  for (const void *q : ps) low |= reinterpret_cast<uintptr_t>(q);
+  return (low & 15) == 0;
+}
+
+}  // namespace rms
+
+template <typename T, bool k8>
+int rms_forward_t(const void *x, const void *r, const void *w, void *y, void *q, float *scale, void *sum, int64_t rows,
+                  int64_t D, double eps, cudaStream_t st) {
+  constexpr int V = 16 / (int)sizeof(T);
+  const rms::FwdArgs<T> p = {static_cast<const T *>(x), static_cast<const T *>(r), static_cast<const T *>(w), static_cast<T *>(y),
+                             static_cast<T *>(sum), q, scale, rows, D, eps};
+  int sms = 0;
+  const int rc = lfw_chunk_sm_count(&sms);
+  if (rc != T2FW_OK) return rc;
+  if (D % V == 0 && rms::aligned({x, r, w, y, q, sum})) return rms::launch_fwd_v<T, V, k8>(p, sms, st);
+  return rms::launch_fwd_v<T, 1, k8>(p, sms, st);
+}
+
+template <typename T>
+int rms_backward_t(const void *dy, const void *dsum, const void *s, const void *w, void *ds, void *dw, int64_t rows, int64_t D,
+                   double eps, void *scratch, cudaStream_t st) {
+  using A = typename Elem<T>::acc;
+  constexpr int V = 16 / (int)sizeof(T);
+  const rms::BwdArgs<T> p = {static_cast<const T *>(dy), static_cast<const T *>(dsum), static_cast<const T *>(s),
+                             static_cast<const T *>(w), static_cast<T *>(ds), static_cast<A *>(scratch), rows, D, eps};
+  int sms = 0;
+  int64_t parts = 0;
+  int rc = lfw_chunk_sm_count(&sms);
+  if (rc != T2FW_OK) return rc;
+  rc = D % V == 0 && rms::aligned({dy, dsum, s, w, ds}) ? rms::launch_bwd_v<T, V>(p, sms, &parts, st)
+                                                        : rms::launch_bwd_v<T, 1>(p, sms, &parts, st);
+  if (rc != T2FW_OK) return rc;
+  T2FW_CHECK_CUDA(launch_dependent(rms::rms_dw_kernel<T>, dim3((unsigned)ceil_div64(D, 32)), dim3(1024), 0, st,
+                                   static_cast<const A *>(scratch), static_cast<T *>(dw), (int)parts, D));
+  T2FW_CHECK_LAUNCH(1);
+  return T2FW_OK;
+}
+
+#define T2FW_RMS_FORWARD(T, k8)                                                                                           \
+  template int rms_forward_t<T, k8>(const void *, const void *, const void *, void *, void *, float *, void *, int64_t,  \
+                                    int64_t, double, cudaStream_t)
+#define T2FW_RMS_BACKWARD(T)                                                                                              \
+  template int rms_backward_t<T>(const void *, const void *, const void *, const void *, void *, void *, int64_t, int64_t, \
+                                 double, void *, cudaStream_t)
+
+}  // namespace t2fw

@@ -6,7 +6,7 @@
 
 Every tensor is multiplied by min(1, max_norm / (total + 1e-6)), the factor of torch.nn.utils.clip_grad_norm_; where that is
 1 the in-place form writes nothing.  Two kernel launches for up to 512 tensors, no synchronisation with the host, sums in
-fp64; total is fp32 (fp64 if a tensor is).  A total that is infinite or NaN goes into the factor as it is.  Tensors may be
+fp64 over vectors of 16 bytes; total is fp32 (fp64 if a tensor is).  A total that is infinite or NaN goes into the factor as it is.  Tensors may be
 of different dtypes; they are dense CUDA tensors of one device, and those that are scaled in place do not share memory.
 """
 import torch
