@@ -11,7 +11,10 @@ namespace t2fw {
 namespace glr {
 
 // V neighbouring channels as they lie in memory: 16 bytes, two 16-bit elements, or one element.
-template <typename T, int V> struct Raw { using type = typename std::conditional<V * sizeof(T) == 16, uint4, uint32_t>::type; };
+template <typename T, int V>
+struct Raw {
+  using type = typename std::conditional<V * sizeof(T) == 16, uint4, typename std::conditional<V * sizeof(T) == 8, uint2, uint32_t>::type>::type;
+};
 template <typename T> struct Raw<T, 1> { using type = T; };
 
 template <typename T, int V, typename A>
@@ -117,10 +120,14 @@ __device__ __forceinline__ void fma_v(A (&r)[V], const A (&a)[V], const A (&b)[V
   }
 }
 
-// ---- asynchronous 16-byte copies into shared memory, and a cluster's shared memory --------------------
+// ---- asynchronous copies into shared memory, and a cluster's shared memory --------------------
 using acp::smem_u32;
-__device__ __forceinline__ void copy16(uint32_t dst, const void *src, bool ok) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(ok ? 16 : 0) : "memory");
+template <int kBytes>      // 16, 8 or 4; zeros where not ok
+__device__ __forceinline__ void copy_in(uint32_t dst, const void *src, bool ok) {
+  if constexpr (kBytes == 16)
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(ok ? 16 : 0) : "memory");
+  else
+    asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(dst), "l"(src), "n"(kBytes), "r"(ok ? kBytes : 0) : "memory");
 }
 __device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>
@@ -158,6 +165,11 @@ __device__ __forceinline__ bool peer_wait(uint64_t *bar, uint32_t parity) {
   }
   return false;
 }
+// Named barriers for n threads: `report` arrives and goes on, `meet` waits for all of them.
+template <int n>
+__device__ __forceinline__ void report(int id) { asm volatile("bar.arrive %0, %1;" ::"r"(id), "n"(n) : "memory"); }
+template <int n>
+__device__ __forceinline__ void meet(int id) { asm volatile("bar.sync %0, %1;" ::"r"(id), "n"(n) : "memory"); }
 // Every thread of every block of the cluster; writes before it are seen behind it.
 __device__ __forceinline__ void cluster_sync() {
   asm volatile("barrier.cluster.arrive.release;\nbarrier.cluster.wait.acquire;" ::: "memory");

@@ -13,8 +13,6 @@
 // backward, from the last step to the first, c = f_{t+1} r_{t+1}, P = f, L = f go, r = go + c.
 #pragma once
 
-#include <cstdlib>
-
 #include "glr.cuh"
 
 namespace t2fw {
@@ -23,7 +21,7 @@ namespace {
 
 using namespace glr;
 
-constexpr int kThreads = 256, kWarps = kThreads / 32, kMaxCluster = 8;
+constexpr int kMaxCluster = 8;
 
 template <typename T>
 struct ScanArgs {
@@ -34,85 +32,120 @@ struct ScanArgs {
   int *status;
 };
 
-// One pass over the data.  A tile is one row b and LW * V channels; a thread holds V of them (16 bytes) over L consecutive
-// steps, LW threads beside one another read a full line, and a block's part of the time axis is kRuns * L steps.  The parts of
-// a round lie on the blocks of a cluster.  Per round: the threads compose their steps into one map, these are composed over
-// the runs of a warp (shuffles), the warps of a block (shared memory) and the blocks of the cluster (each writes its map into
-// the others' shared memory), and with the carry thus known at its start every thread walks its steps again from registers.
+// One pass over the data.  A tile is one row b and LW * V channels; a thread holds V of them over L consecutive steps, LW threads
+// beside one another read a line of memory, and a block's part of the time axis is kRuns * L steps.  The parts of a round lie on
+// the blocks of a cluster.  Per round
+//   A  every thread composes its steps into one map c -> P c + S, and these are composed over the runs of a warp (shuffles)
+//   B  the maps are composed over the warps of a block (shared memory) and sent to the other blocks of the cluster
+//   C  with the maps of all blocks, what is carried into each warp's steps is known
+//   D  every thread walks its steps again and writes its results
+// B and C are the work of one more warp.  The others come to D of a round only after A of the next one, so that warp has the
+// time of a round, and they meet it at named barriers: they report their maps and go on, and find what is carried in when they
+// need it.  Maps and carried values alternate between two halves.
 // Each thread copies what it alone will read, `kStages` rounds ahead, so the copies need no barrier.
-template <typename T, int V, int LW, bool kFused, bool kBwd, int L, int kStages>
-__global__ void __launch_bounds__(kThreads, V * sizeof(T) == 16 ? 2 : 3)
+template <typename T, int V, int LW, bool kFused, bool kBwd, int L, int kStages, int kThreads, int kMin>
+__global__ void __launch_bounds__(kThreads + 32, kMin)
 glr_scan_kernel(const ScanArgs<T> p) {
   using A = typename Elem<T>::acc;
   using R = typename Raw<T, V>::type;
   using A2 = typename Pair<A>::type;
-  constexpr bool kAsync = V * sizeof(T) == 16, kFast = sizeof(T) == 2;
+  constexpr int kBytes = V * (int)sizeof(T), kWarps = kThreads / 32;
+  constexpr bool kAsync = kBytes >= 4, kFast = sizeof(T) == 2;
   constexpr int kRuns = kThreads / LW, kPart = kRuns * L, CH = LW * V;
   constexpr int NT = kBwd ? (kFused ? 4 : 3) : 2;      // arrays read: fwd x, f; bwd go, f, h, (v)
-  constexpr uint32_t kSlot = NT * L * kThreads * 16;
+  constexpr uint32_t kLine = kThreads * kBytes, kSlot = NT * L * kLine;
   extern __shared__ __align__(16) unsigned char ring[];
-  __shared__ __align__(16) A2 s_map[kWarps][CH];       // (P, S) of a warp's steps
-  __shared__ __align__(16) A s_in[kWarps][CH];         // what is carried into a warp's steps
+  __shared__ __align__(16) A2 s_map[2][kWarps][CH];    // (P, S) of a warp's steps
+  __shared__ __align__(16) A s_in[2][kWarps][CH];      // what is carried into a warp's steps
   __shared__ __align__(8) uint64_t bar[2];
-  A2 *const s_peer = reinterpret_cast<A2 *>(ring + (kAsync ? kStages * kSlot : 0));      // [2][C][CH]: maps from the cluster's blocks
+  constexpr int K = (CH + 31) / 32, kMaps = 1, kIns = 3;      // channels per thread of the last warp; numbers of named barriers
+  A2 *const s_peer = reinterpret_cast<A2 *>(ring + kStages * kSlot);      // [2][C][CH]: maps from the cluster's blocks
   dependency_wait();
 
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int col = tid % LW, run = tid / LW;
-  const int C = p.cluster, rank = C > 1 ? (int)(blockIdx.x % (unsigned)C) : 0;
+  const int C = p.cluster, N = p.iterations, rank = C > 1 ? (int)(blockIdx.x % (unsigned)C) : 0;
   const unsigned tile = blockIdx.x / (unsigned)C;
   const int64_t b = tile / (unsigned)p.tiles, d0 = (int64_t)(tile % (unsigned)p.tiles) * CH;
   const int64_t d = d0 + col * V, D = p.D, steps = p.T_, row = kFused ? 2 * D : D;
   const bool on = d < D;
-  const T *const px = p.x + b * steps * row + d, *const pf = kFused ? px + D : p.f + b * steps * D + d;
-  const T *const pgo = kBwd ? p.go + b * steps * D + d : nullptr, *const pho = kBwd ? p.out_in + b * steps * D + d : nullptr;
+  // Steps are counted in walking order: tau = t forward, steps - 1 - t backward.  Addresses of this thread's first step in the
+  // round that is fetched next and in the round that is written next; from step to step and from round to round they move by
+  // the same distance.
+  const int64_t hop = (int64_t)C * kPart, tau_first = (int64_t)rank * kPart + run * L, t_first = kBwd ? steps - 1 - tau_first : tau_first;
+  const int64_t one = kBwd ? -1 : 1, wide = one * row, narrow = one * D;      // a step in arrays of width `row` and of width D
+  const T *in[NT];
+  {
+    const int64_t at = (b * steps + t_first) * D + d, at_row = (b * steps + t_first) * row + d;
+    if constexpr (!kBwd) {
+      in[0] = p.x + at_row;
+      in[1] = kFused ? p.x + at_row + D : p.f + at;
+    } else {
+      in[0] = p.go + at;
+      in[1] = kFused ? p.x + at_row + D : p.f + at;
+      in[2] = p.out_in + at - D;
+      if constexpr (kFused) in[NT - 1] = p.x + at_row;
+    }
+  }
+  T *out0 = p.out + (b * steps + t_first) * (kBwd ? row : D) + d, *out1 = nullptr;
+  if constexpr (kBwd) out1 = kFused ? out0 + D : p.df + (b * steps + t_first) * D + d;
   const T *const pst = p.state + b * D + d;
-
-  // Address of array j's values for step t.
-  auto source = [&](int j, int64_t t) -> const T * {
-    if constexpr (!kBwd) return j == 0 ? px + t * row : pf + t * row;
-    if (j == 0) return pgo + t * D;
-    if (j == 1) return pf + t * row;
-    if (j == 2) return t > 0 ? pho + (t - 1) * D : pst;
-    return px + t * row;
+  // of L steps, how many lie before the end (any number of them: no more than 2^30 is told apart)
+  auto room = [&](int64_t tau) {
+    const int64_t n = steps - tau;
+    return !on || n < 0 ? 0 : n > (1 << 30) ? 1 << 30 : (int)n;
   };
+  int64_t tau_fetch = tau_first, tau_write = tau_first;
+  R held_back[kAsync ? 1 : NT][kAsync ? 1 : L];      // single 16-bit values cannot be copied asynchronously: fetched into registers
   auto fetch = [&](int it) {
-    if constexpr (kAsync) {
-      const int64_t tau0 = ((int64_t)it * C + rank) * kPart + run * L;      // in walking order
-      const uint32_t slot = smem_u32(ring) + (uint32_t)(it % kStages) * kSlot + tid * 16;
-      if (it < p.iterations) {
+    if (it < N) {
+      const int left = room(tau_fetch);
+      const uint32_t slot = smem_u32(ring) + (uint32_t)(it % kStages) * kSlot + tid * kBytes;
+#pragma unroll
+      for (int j = 0; j < NT; ++j) {
+        const int64_t step = kFused && (!kBwd || j == 1 || j == 3) ? wide : narrow;
+        const T *q = in[j];
 #pragma unroll
         for (int i = 0; i < L; ++i) {
-          const int64_t tau = tau0 + i, t = kBwd ? steps - 1 - tau : tau;
-          const bool ok = on && tau < steps;
-#pragma unroll
-          for (int j = 0; j < NT; ++j) copy16(slot + (j * L + i) * (kThreads * 16), ok ? source(j, t) : p.state, ok);
+          const bool ok = i < left;
+          const T *from = ok ? q : p.state;
+          if (kBwd && j == 2 && i == left - 1 && left < (1 << 30)) from = pst;      // before the first step lies the state
+          if constexpr (kAsync) {
+            copy_in<kBytes>(slot + (j * L + i) * kLine, from, ok);
+          } else {
+            held_back[j][i] = R{};
+            if (ok) held_back[j][i] = *reinterpret_cast<const R *>(from);
+          }
+          q += step;
         }
+        in[j] += hop * step;
       }
-      copy_commit();
+      tau_fetch += hop;
     }
+    copy_commit();
   };
-  auto value = [&](int it, int j, int i, A (&v)[V]) {
-    if constexpr (kAsync) {
-      unpack<T, V>(*reinterpret_cast<const R *>(ring + (uint32_t)(it % kStages) * kSlot + (j * L + i) * (kThreads * 16) + tid * 16), v);
-    } else {
-      const int64_t tau = ((int64_t)it * C + rank) * kPart + run * L + i, t = kBwd ? steps - 1 - tau : tau;
-      R u = {};
-      if (on && tau < steps) u = *reinterpret_cast<const R *>(source(j, t));
-      unpack<T, V>(u, v);
-    }
+  auto raw = [&](int it, int j, int i) -> R & {
+    return *reinterpret_cast<R *>(ring + (uint32_t)(it % kStages) * kSlot + (j * L + i) * kLine + tid * kBytes);
   };
-
+  auto put = [&](int it) {      // what `fetch` left in registers
+    if constexpr (!kAsync) {
 #pragma unroll
-  for (int s = 0; s < kStages; ++s) fetch(s);
-  // the thread of a channel keeps what is carried from round to round
-  A carry = A(0);
-  if (tid < CH && d0 + tid < D) {
-    if constexpr (!kBwd) carry = (A)Elem<T>::ld(p.state + b * D + d0 + tid);
-    else if (p.gs != nullptr) carry = (A)Elem<T>::ld(p.gs + b * D + d0 + tid);
-  }
+      for (int j = 0; j < NT; ++j)
+#pragma unroll
+        for (int i = 0; i < L; ++i) raw(it, j, i) = held_back[j][i];
+    }
+  };
+  // step i of this thread in round `it`: x (or go), the gate and 1 - gate
+  auto values = [&](int it, int i, A (&u)[V], A (&f)[V], A (&rest)[V]) {
+    unpack<T, V>(raw(it, 0, i), u);
+    unpack<T, V>(raw(it, 1, i), f);
+    if constexpr (kFused) {
+#pragma unroll
+      for (int k = 0; k < V; ++k) gate_pair<kFast>(f[k], f[k], rest[k]);
+      if constexpr (!kBwd) mul_v(u, u, rest);
+    }
+  };
 
-  bool gave_up = false;
   if (C > 1) {      // the other blocks' barriers and shared memory are there to be written to
     if (tid == 0) {
       acp::mbar_init(&bar[0], 1);
@@ -121,158 +154,223 @@ glr_scan_kernel(const ScanArgs<T> p) {
     }
     cluster_sync();
   }
-  for (int it = 0; it < p.iterations; ++it) {
-    if constexpr (kAsync) copy_wait<kStages - 1>();
-    const int64_t tau0 = ((int64_t)it * C + rank) * kPart + run * L;
-    A u[L][V], f[L][V], rest[kFused && kBwd ? L : 1][V];      // x (or go), the gate, 1 - gate
-    const bool ragged = ((int64_t)it * C + rank + 1) * kPart > steps;
-    A P[V], S[V];      // the composed map of this thread's steps, then of all runs of the warp up to it
+  if (warp == kWarps) {      // B and C
+    A carry[K];
 #pragma unroll
-    for (int i = 0; i < L; ++i) {
-      value(it, 0, i, u[i]);
-      value(it, 1, i, f[i]);
-      if constexpr (kFused) {
-#pragma unroll
-        for (int k = 0; k < V; ++k) gate_pair<kFast>(f[i][k], f[i][k], rest[kBwd ? i : 0][k]);
-        if constexpr (!kBwd) mul_v(u[i], u[i], rest[0]);
-      }
-      if (ragged && tau0 + i >= steps) {      // behind the end a step changes nothing
-#pragma unroll
-        for (int k = 0; k < V; ++k) f[i][k] = A(1), u[i][k] = A(0);
-      }
-      if (i == 0) {
-#pragma unroll
-        for (int k = 0; k < V; ++k) P[k] = f[0][k];
-        // the state before the first step is zero: f * 0 keeps an infinite or NaN gate in sight
-        A zero[V];
-#pragma unroll
-        for (int k = 0; k < V; ++k) zero[k] = A(0);
-        if constexpr (kBwd) mul_v(S, f[0], u[0]);
-        else fma_v(S, f[0], zero, u[0]);
-      } else {
-        mul_v(P, P, f[i]);
-        if constexpr (kBwd) {
-#pragma unroll
-          for (int k = 0; k < V; ++k) S[k] += u[i][k];
-          mul_v(S, S, f[i]);
-        } else {
-          fma_v(S, f[i], S, u[i]);
-        }
+    for (int k = 0; k < K; ++k) {
+      const int64_t at = d0 + lane + 32 * k;
+      carry[k] = A(0);
+      if (lane + 32 * k < CH && at < D) {
+        if constexpr (!kBwd) carry[k] = (A)Elem<T>::ld(p.state + b * D + at);
+        else if (p.gs != nullptr) carry[k] = (A)Elem<T>::ld(p.gs + b * D + at);
       }
     }
+    bool gave_up = false;
+    for (int it = 0; it < N; ++it) {
+      const int h = it & 1;
+      meet<kThreads + 32>(kMaps + h);
+      A2 m[K][kWarps];
+      A start[K];
 #pragma unroll
-    for (int k = 0; k < V; ++k) P[k] = held(P[k]);
-    if constexpr (LW < 32) {
+      for (int k = 0; k < K; ++k) {
 #pragma unroll
-      for (int o = LW; o < 32; o <<= 1) {
-        A Pp[V], Sp[V];
-#pragma unroll
-        for (int k = 0; k < V; ++k) {
-          Pp[k] = __shfl_up_sync(0xffffffffu, P[k], o);
-          Sp[k] = __shfl_up_sync(0xffffffffu, S[k], o);
-        }
-        if (lane >= o) {
-          fma_v(S, P, Sp, S);
-          mul_v(P, P, Pp);
-#pragma unroll
-          for (int k = 0; k < V; ++k) P[k] = held(P[k]);
-        }
-      }
-    }
-    if (lane >= 32 - LW) {
-#pragma unroll
-      for (int k = 0; k < V; ++k) s_map[warp][col * V + k] = A2{P[k], S[k]};
-    }
-    __syncthreads();
-    A2 m[kWarps];
-    A start = carry;
-    if (tid < CH) {
-      A Pb = A(1), Sb = A(0);
-#pragma unroll
-      for (int w = 0; w < kWarps; ++w) m[w] = s_map[w][tid];
-#pragma unroll
-      for (int w = 0; w < kWarps; ++w) {
-        Sb = m[w].x * Sb + m[w].y;
-        Pb = held(Pb * m[w].x);
+        for (int w = 0; w < kWarps; ++w)
+          if (lane + 32 * k < CH) m[k][w] = s_map[h][w][lane + 32 * k];
       }
       if (C == 1) {
-        carry = Pb * carry + Sb;
+#pragma unroll
+        for (int k = 0; k < K; ++k) start[k] = carry[k];
       } else {
-        // The maps of a round go into the half of the round before last.  A block sends those of this round only after it has
-        // got all of the last round, and each block sent those after it had read the round before.
-        if (tid == 0) acp::mbar_expect_tx(&bar[it & 1], (uint32_t)(C * CH * sizeof(A2)));
-        A2 *const half = s_peer + (it & 1) * C * CH;
-        const uint32_t at = smem_u32(half + rank * CH + tid), sem = smem_u32(&bar[it & 1]);
-        for (int r = 0; r < C; ++r) peer_send(peer_address(at, r), A2{Pb, Sb}, peer_address(sem, r));
-        if (!gave_up) gave_up = !peer_wait(&bar[it & 1], (it >> 1) & 1);
-        A2 q[kMaxCluster];
+        // The maps of a round go into the half of the round before last.  A block sends them after it has the maps of all blocks
+        // of the last round, and each block sent those after it had read the half.
+        if (lane == 0) acp::mbar_expect_tx(&bar[h], (uint32_t)(C * CH * sizeof(A2)));
+        A2 *const half = s_peer + h * C * CH;
 #pragma unroll
-        for (int r = 0; r < kMaxCluster; ++r)
-          if (r < C) q[r] = half[r * CH + tid];
+        for (int k = 0; k < K; ++k) {
+          A Pb = A(1), Sb = A(0);
 #pragma unroll
-        for (int r = 0; r < kMaxCluster; ++r)
-          if (r < C) {
-            if (r == rank) start = carry;
-            carry = q[r].x * carry + q[r].y;
+          for (int w = 0; w < kWarps; ++w) {
+            Sb = m[k][w].x * Sb + m[k][w].y;
+            Pb = held(Pb * m[k][w].x);
           }
-      }
-#pragma unroll
-      for (int w = 0; w < kWarps; ++w) {
-        s_in[w][tid] = start;
-        start = m[w].x * start + m[w].y;
-      }
-    }
-    __syncthreads();
-    A c[V], behind[V];
-#pragma unroll
-    for (int k = 0; k < V; ++k) c[k] = s_in[warp][col * V + k];
-    if constexpr (LW < 32) {      // what the run before leaves is what enters this one
-      fma_v(behind, P, c, S);
-#pragma unroll
-      for (int k = 0; k < V; ++k) {
-        const A q = __shfl_up_sync(0xffffffffu, behind[k], LW);
-        if (lane >= LW) c[k] = q;
-      }
-    }
-#pragma unroll
-    for (int i = 0; i < L; ++i) {
-      const int64_t tau = tau0 + i, t = kBwd ? steps - 1 - tau : tau;
-      const bool write = on && tau < steps;
-      if constexpr (!kBwd) {
-        fma_v(c, f[i], c, u[i]);
-        if (write) *reinterpret_cast<R *>(p.out + (b * steps + t) * D + d) = pack<T, V>(c);
-      } else {
-        A before[V], r[V];
-        value(it, 2, i, before);
-#pragma unroll
-        for (int k = 0; k < V; ++k) r[k] = u[i][k] + c[k];
-        mul_v(c, f[i], r);
-        if constexpr (kFused) {
-          A v[V];
-          value(it, 3, i, v);
-          mul_v(r, r, rest[i]);      // d_v
-#pragma unroll
-          for (int k = 0; k < V; ++k) v[k] = f[i][k] * r[k] * (before[k] - v[k]);      // d_g
-          if (write) {
-            T *to = p.out + (b * steps + t) * row + d;
-            *reinterpret_cast<R *>(to) = pack<T, V>(r);
-            *reinterpret_cast<R *>(to + D) = pack<T, V>(v);
+          if (lane + 32 * k < CH) {
+            const uint32_t at = smem_u32(half + rank * CH + lane + 32 * k), sem = smem_u32(&bar[h]);
+            for (int r = 0; r < C; ++r) peer_send(peer_address(at, r), A2{Pb, Sb}, peer_address(sem, r));
           }
+        }
+        if (!gave_up) gave_up = !peer_wait(&bar[h], (it >> 1) & 1);
+#pragma unroll
+        for (int k = 0; k < K; ++k) {
+          start[k] = carry[k];
+          A2 q[kMaxCluster];
+#pragma unroll
+          for (int r = 0; r < kMaxCluster; ++r)
+            if (r < C && lane + 32 * k < CH) q[r] = half[r * CH + lane + 32 * k];
+#pragma unroll
+          for (int r = 0; r < kMaxCluster; ++r)
+            if (r < C) {
+              if (r == rank) start[k] = carry[k];
+              carry[k] = q[r].x * carry[k] + q[r].y;
+            }
+        }
+      }
+#pragma unroll
+      for (int k = 0; k < K; ++k) {
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) {
+          if (lane + 32 * k < CH) s_in[h][w][lane + 32 * k] = start[k];
+          start[k] = m[k][w].x * start[k] + m[k][w].y;
+        }
+        if (C == 1) carry[k] = start[k];
+      }
+      report<kThreads + 32>(kIns + h);
+    }
+    if (gave_up) atomicExch(p.status, 1);
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      const int64_t at = d0 + lane + 32 * k;
+      if (rank == 0 && lane + 32 * k < CH && at < D) Elem<T>::st(p.end + b * D + at, carry[k]);
+    }
+    if (C > 1) cluster_sync();      // no block leaves while another may still send to it
+    return;
+  }
+
+  if constexpr (kAsync) {
+#pragma unroll
+    for (int s = 0; s < kStages; ++s) fetch(s);
+  } else {
+    fetch(0);
+    put(0);
+    fetch(1);
+  }
+  A P[V], S[V], P0[V], S0[V];
+  for (int it = 0;; ++it) {
+    if (it < N) {      // A
+      if constexpr (kAsync) {
+        if (it == 0) copy_wait<kStages - 1>();
+        else copy_wait<kStages - 2>();
+      }
+      const bool ragged = ((int64_t)it * C + rank + 1) * kPart > steps;
+      const int64_t tau0 = ((int64_t)it * C + rank) * kPart + run * L;
+#pragma unroll
+      for (int i = 0; i < L; ++i) {
+        A u[V], f[V], rest[V];
+        values(it, i, u, f, rest);
+        if (ragged && tau0 + i >= steps) {      // behind the end a step changes nothing
+#pragma unroll
+          for (int k = 0; k < V; ++k) f[k] = A(1), u[k] = A(0);
+        }
+        if (i == 0) {
+          // before the first step the state is zero: f * 0 keeps an infinite or NaN gate in sight
+          A zero[V];
+#pragma unroll
+          for (int k = 0; k < V; ++k) P[k] = f[k], zero[k] = A(0);
+          if constexpr (kBwd) mul_v(S, f, u);
+          else fma_v(S, f, zero, u);
         } else {
-          mul_v(before, before, r);
-          if (write) {
-            *reinterpret_cast<R *>(p.out + (b * steps + t) * D + d) = pack<T, V>(r);
-            *reinterpret_cast<R *>(p.df + (b * steps + t) * D + d) = pack<T, V>(before);
+          mul_v(P, P, f);
+          if constexpr (kBwd) {
+#pragma unroll
+            for (int k = 0; k < V; ++k) S[k] += u[k];
+            mul_v(S, S, f);
+          } else {
+            fma_v(S, f, S, u);
           }
         }
       }
+#pragma unroll
+      for (int k = 0; k < V; ++k) P[k] = held(P[k]);
+      if constexpr (LW < 32) {
+#pragma unroll
+        for (int o = LW; o < 32; o <<= 1) {
+          A Pp[V], Sp[V];
+#pragma unroll
+          for (int k = 0; k < V; ++k) {
+            Pp[k] = __shfl_up_sync(0xffffffffu, P[k], o);
+            Sp[k] = __shfl_up_sync(0xffffffffu, S[k], o);
+          }
+          if (lane >= o) {
+            fma_v(S, P, Sp, S);
+            mul_v(P, P, Pp);
+#pragma unroll
+            for (int k = 0; k < V; ++k) P[k] = held(P[k]);
+          }
+        }
+      }
+      if (lane >= 32 - LW) {
+#pragma unroll
+        for (int k = 0; k < V; ++k) s_map[it & 1][warp][col * V + k] = A2{P[k], S[k]};
+      }
+      report<kThreads + 32>(kMaps + (it & 1));
     }
-    fetch(it + kStages);
+    if (it > 0) {      // D, of the round before
+      const int e = it - 1;
+      meet<kThreads + 32>(kIns + (e & 1));
+      const int left = room(tau_write);
+      T *w0 = out0, *w1 = out1;
+      A c[V];
+#pragma unroll
+      for (int k = 0; k < V; ++k) c[k] = s_in[e & 1][warp][col * V + k];
+      if constexpr (LW < 32) {      // what the run before leaves is what enters this one
+        A behind[V];
+        fma_v(behind, P0, c, S0);
+#pragma unroll
+        for (int k = 0; k < V; ++k) {
+          const A q = __shfl_up_sync(0xffffffffu, behind[k], LW);
+          if (lane >= LW) c[k] = q;
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < L; ++i) {
+        const bool write = i < left;
+        A u[V], f[V], rest[V];
+        values(e, i, u, f, rest);
+        if constexpr (!kBwd) {
+          fma_v(c, f, c, u);
+          if (write) *reinterpret_cast<R *>(w0) = pack<T, V>(c);
+          w0 += D;
+        } else {
+          A before[V];
+          unpack<T, V>(raw(e, 2, i), before);
+#pragma unroll
+          for (int k = 0; k < V; ++k) u[k] += c[k];      // r
+          mul_v(c, f, u);
+          if constexpr (kFused) {
+            A v[V];
+            unpack<T, V>(raw(e, NT - 1, i), v);
+            mul_v(u, u, rest);      // d_v
+#pragma unroll
+            for (int k = 0; k < V; ++k) v[k] = f[k] * u[k] * (before[k] - v[k]);      // d_g
+            if (write) {
+              *reinterpret_cast<R *>(w0) = pack<T, V>(u);
+              *reinterpret_cast<R *>(w1) = pack<T, V>(v);
+            }
+          } else {
+            mul_v(before, before, u);
+            if (write) {
+              *reinterpret_cast<R *>(w0) = pack<T, V>(u);
+              *reinterpret_cast<R *>(w1) = pack<T, V>(before);
+            }
+          }
+          w0 += wide;
+          w1 += wide;
+        }
+      }
+      tau_write += hop;
+      out0 += hop * (kBwd ? wide : D);
+      if constexpr (kBwd) out1 += hop * wide;
+      if constexpr (kAsync) fetch(e + kStages);
+    }
+    if (it == N) break;
+    if constexpr (!kAsync) {
+      put(it + 1);
+      fetch(it + 2);
+    }
+#pragma unroll
+    for (int k = 0; k < V; ++k) P0[k] = P[k], S0[k] = S[k];
   }
-  if constexpr (kAsync) copy_wait<0>();
-  if (gave_up) atomicExch(p.status, 1);
-  if (C > 1) cluster_sync();      // no block leaves while another may still send to it
-  if (rank == 0 && tid < CH && d0 + tid < D) Elem<T>::st(p.end + b * D + d0 + tid, carry);
+  copy_wait<0>();
+  if (C > 1) cluster_sync();
 }
 
 // Every thread walks V channels of a row from the first step to the last, U steps' loads at a time, the next U on their way:
@@ -283,7 +381,7 @@ glr_walk_kernel(const ScanArgs<T> p, int64_t n) {
   using A = typename Elem<T>::acc;
   using R = typename Raw<T, V>::type;
   constexpr bool kFast = sizeof(T) == 2;
-  constexpr int U = sizeof(R) < 16 ? 8 : kBwd ? 2 : 4, NT = kBwd ? (kFused ? 4 : 3) : 2;
+  constexpr int U = sizeof(R) < 16 ? 8 : !kBwd ? 6 : kFused ? 3 : 4, NT = kBwd ? (kFused ? 4 : 3) : 2;
   dependency_wait();
   const int64_t i0 = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
   if (i0 >= n) return;
@@ -367,25 +465,25 @@ glr_walk_kernel(const ScanArgs<T> p, int64_t n) {
   *reinterpret_cast<R *>(p.end + at) = pack<T, V>(c);
 }
 
-template <typename T, int V, int LW, bool kFused, bool kBwd, int L, int kStages>
-int launch_scan_v(ScanArgs<T> p, int64_t B, int sms, cudaStream_t st, int forced = 0, int pad = 0) {
-  constexpr bool kAsync = V * sizeof(T) == 16;
+template <typename T, int V, int LW, bool kFused, bool kBwd, int L, int kStages, int kThreads, int kMin>
+int launch_scan_v(ScanArgs<T> p, int64_t B, int sms, cudaStream_t st) {
   constexpr int kPart = kThreads / LW * L, CH = LW * V;
   constexpr int NT = kBwd ? (kFused ? 4 : 3) : 2;
-  constexpr size_t ring = kAsync ? (size_t)kStages * NT * L * kThreads * 16 : 0, map = CH * 2 * sizeof(typename Elem<T>::acc);
-  const auto kernel = &glr_scan_kernel<T, V, LW, kFused, kBwd, L, kStages>;
+  constexpr size_t ring = (size_t)kStages * NT * L * kThreads * V * sizeof(T), map = CH * 2 * sizeof(typename Elem<T>::acc);
+  const auto kernel = &glr_scan_kernel<T, V, LW, kFused, kBwd, L, kStages, kThreads, kMin>;
   static std::atomic<unsigned long long> ready{0};
   int dev = 0;
   T2FW_CHECK_CUDA(cudaGetDevice(&dev));
   if (!(ready.load(std::memory_order_relaxed) >> (dev & 63) & 1)) {
     T2FW_CHECK_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                         pad ? 200000 : (int)(ring + 2 * kMaxCluster * map)));
+                                         220 * 1024 - (int)(2 * (kThreads / 32) * (map + map / 2))));
     ready.fetch_or(1ull << (dev & 63), std::memory_order_relaxed);
   }
   const int64_t tiles = ceil_div64(p.D, CH), all = B * tiles, parts = ceil_div64(p.T_, kPart);
+  // Blocks per tile: enough for every SM to have one (backward), or one and a half (forward).  Forward with clusters of 2 / 4 / 8,
+  // us: 8 x 1024 x 768 15.0 / 12.3 / 15.7, 3 x 777 x 1016 10.7 / 9.4 / 8.4; backward 18.9 / 21.5 / 23.2 and 12.5 / 11.4 / 14.3.
   int C = 1;
-  while (C < kMaxCluster && C < parts && all * C < 2 * sms) C *= 2;
-  if (forced) C = forced < parts ? forced : (int)parts;
+  while (C < kMaxCluster && C < parts && all * C < (kBwd ? sms : sms + sms / 2)) C *= 2;
   T2FW_CHECK_ARG(tiles <= 0x7fffffff && all <= 0x7fffffff / C && parts <= 0x7fffffff, "sizes out of range");
   p.tiles = (int)tiles;
   p.cluster = C;
@@ -394,9 +492,14 @@ int launch_scan_v(ScanArgs<T> p, int64_t B, int sms, cudaStream_t st, int forced
   if (rc != T2FW_OK) return rc;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(all * C));
-  cfg.blockDim = dim3(kThreads);
+  cfg.blockDim = dim3(kThreads + 32);
+  // Blocks of a cluster are placed side by side, as many to an SM as fit, while other SMs stay empty: ask for so much shared
+  // memory that no more fit than the launch has per SM (1 x 65536 x 1024 forward 146 -> 107 us), or two: with one, clusters of
+  // eight did not all find room at once (268 us where two fit 186).
+  constexpr size_t fixed = 2 * (kThreads / 32) * (map + map / 2) + 1024 + 16, per_sm = 228 * 1024;
+  const size_t k = all * C > 2 * sms ? (size_t)ceil_div64(all * C, sms) : 2, spread = per_sm / (k + 1) + 1;
   cfg.dynamicSmemBytes = ring + (C > 1 ? 2 * C * map : 0);
-  if (pad) cfg.dynamicSmemBytes = 120000 > cfg.dynamicSmemBytes ? 120000 : cfg.dynamicSmemBytes;
+  if (C > 1 && cfg.dynamicSmemBytes + fixed < spread) cfg.dynamicSmemBytes = (spread - fixed + 15) / 16 * 16;
   cfg.stream = st;
   cudaLaunchAttribute attr[2];
   int n = 0;
@@ -419,20 +522,33 @@ int launch_scan_v(ScanArgs<T> p, int64_t B, int sms, cudaStream_t st, int forced
   return T2FW_OK;
 }
 
-template <typename T, int V, int LW, bool kFused, bool kBwd, int L, int kStages>
+template <typename T, int V, bool kFused, bool kBwd>
 int launch_v(const ScanArgs<T> &p, int64_t B, cudaStream_t st) {
   int sms = 0;
   const int rc = lfw_chunk_sm_count(&sms);
   if (rc != T2FW_OK) return rc;
   const int64_t n = B * p.D / V;
-  static const int walk = std::getenv("GLR_WALK") ? std::atoi(std::getenv("GLR_WALK")) : -1;
-  if (walk >= 0 ? walk : p.T_ <= 32 || n >= 128 * sms) {
+  // Walkers need many channels or few steps.  Scan against walk, forward, bf16, us: 256 x 64 steps x 768 (24 576 walkers) 20.7 /
+  // 16.7, 128 x 64 x 768 11.4 / 13.6, 512 x 128 x 1024 81.0 / 80.8 (backward 131 / 108), 256 x 16 x 768 17.7 / 5.3,
+  // 64 x 40 x 768 6.1 / 9.1, 16 x 24 x 512 2.1 / 3.3.
+  if (p.T_ <= 8 || n >= 128 * sms || (n >= 40 * sms && p.T_ <= 32)) {
+    T2FW_CHECK_ARG(n <= 128 * (int64_t)0x7fffffff, "sizes out of range");
     T2FW_CHECK_CUDA(launch_dependent(glr_walk_kernel<T, V, kFused, kBwd>, dim3((unsigned)ceil_div64(n, 128)), dim3(128), 0, st,
                                      p, n));
     T2FW_CHECK_LAUNCH(1);
     return T2FW_OK;
   }
-  return launch_scan_v<T, V, LW, kFused, kBwd, L, kStages>(p, B, sms, st);
+  if constexpr (V * sizeof(T) == 16) {
+    constexpr int kMin = kFused && kBwd ? 2 : 3;
+    // Full lines, or half lines where those tiles are so few that a cluster each leaves SMs without work.  Full against half,
+    // bf16, us, forward and backward: 1 x 65536 x 1024 (16 tiles) 268 / 107 and 324 / 146, 4 x 4096 x 512 (32) 16.1 / 16.6 and
+    // 20.9 / 22.0, 64 x 1024 x 1024 76 / 83 and 122 / 130.
+    if (B * ceil_div64(p.D, 8 * V) * kMaxCluster >= sms + sms / 2)
+      return launch_scan_v<T, V, 8, kFused, kBwd, 4, 3, 128, kMin>(p, B, sms, st);
+    return launch_scan_v<T, V, 4, kFused, kBwd, 4, 3, 128, kMin>(p, B, sms, st);
+  } else {
+    return launch_scan_v<T, V, 32, kFused, kBwd, 8, 3, 256, 2>(p, B, sms, st);
+  }
 }
 
 // 16 bytes per thread where rows and pointers allow them, else a 32-bit word, else an element.
@@ -442,11 +558,10 @@ int launch_scan(const ScanArgs<T> &p, int64_t B, cudaStream_t st) {
   const void *const ptr[] = {p.x, p.f, p.go, p.gs, p.out_in, p.state, p.out, p.df, p.end};
   uintptr_t low = 0;
   for (const void *q : ptr) low |= reinterpret_cast<uintptr_t>(q);
-  if (p.D % V == 0 && (low & 15) == 0)
-    return launch_v<T, V, 8, kFused, kBwd, kBwd && kFused ? 2 : 4, kBwd ? 2 : 3>(p, B, st);
+  if (p.D % V == 0 && (low & 15) == 0) return launch_v<T, V, kFused, kBwd>(p, B, st);
   if constexpr (sizeof(T) == 2)
-    if (p.D % 2 == 0 && (low & 3) == 0) return launch_v<T, 2, 32, kFused, kBwd, 8, 1>(p, B, st);
-  return launch_v<T, 1, 32, kFused, kBwd, 8, 1>(p, B, st);
+    if (p.D % 2 == 0 && (low & 3) == 0) return launch_v<T, 2, kFused, kBwd>(p, B, st);
+  return launch_v<T, 1, kFused, kBwd>(p, B, st);
 }
 
 }  // namespace
