@@ -85,8 +85,11 @@ def parse_args():
                         "BASELINE config 4 names 128)")
     p.add_argument("--scaling", default="weak", choices=["weak", "strong"],
                    help="weak: every GPU runs the workload's batch rows; strong: the rows are split over the GPUs")
-    p.add_argument("--rule", default="dfw", choices=["dfw", "lfw"],
+    p.add_argument("--rule", default="dfw", choices=["dfw", "lfw", "glr"],
                    help="recurrence inside the gpt2 workload's attention replacement")
+    p.add_argument("--norm", default="layer", choices=["layer", "rms"], help="norms of the gpt2 workload's model")
+    p.add_argument("--clip-grad", type=float, default=0.0,
+                   help="clip the gpt2 workload's gradients to this global norm before the optimizer step (0: off)")
     p.add_argument("--graph", default="auto", choices=["auto", "on", "off"],
                    help="replay the K timed steps as one CUDA graph (auto: on)")
     return p.parse_args()
@@ -285,11 +288,12 @@ def run_gpt2(args):
         dist.init_process_group("nccl", device_id=dev)
     from t2fw_b200 import _lib
     from t2fw_b200.gpt2_fw import GPT2FW, GPT2FWConfig
+    from t2fw_b200.grad_clip import clip_grad_norm_
     from t2fw_b200.parallel import job_throughput, max_over_ranks
 
     lib = _lib.load_core()
     torch.manual_seed(args.seed)                       # same initial weights on every rank
-    cfg = GPT2FWConfig(rule=args.rule)
+    cfg = GPT2FWConfig(rule=args.rule, norm=args.norm)
     model = GPT2FW(cfg).half().to(dev)
     n_params = model.n_params()
     net = model
@@ -304,6 +308,8 @@ def run_gpt2(args):
     def step(ids):
         loss = net(ids[:, :-1], targets=ids[:, 1:])
         loss.backward()
+        if args.clip_grad > 0:
+            clip_grad_norm_(net.parameters(), args.clip_grad)
         opt.step()
         opt.zero_grad(set_to_none=True)
         return loss
@@ -368,7 +374,9 @@ def run_gpt2(args):
         "data": "synthetic",
         "config": {"workload": "gpt2: GPT-2-small (12 layers, d_model 768, 12 heads, %.1f M parameters, random init), "
                                "every attention replaced by a %s layer, seq 1024, batch 8 per GPU, uniform random "
-                               "token ids; forward + backward + AdamW" % (n_params / 1e6, args.rule.upper()),
+                               "token ids; forward + backward + AdamW" % (n_params / 1e6, args.rule.upper()) +
+                               (", root-mean-square norms" if args.norm == "rms" else "") +
+                               (", gradients clipped to %g" % args.clip_grad if args.clip_grad > 0 else ""),
                    "parallelism": "dp%d (DistributedDataParallel, NCCL all-reduce of gradients)" % world,
                    "l2": "activations of a step (several GB) are larger than L2",
                    "loss_first": first, "loss_last": last},

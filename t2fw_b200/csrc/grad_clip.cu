@@ -12,7 +12,7 @@ namespace t2fw {
 
 namespace {
 
-constexpr int kTable = 512, kThreads = 256, kPieceBytes = 32768, kVectors = kPieceBytes / (16 * kThreads), kMaxBlocks = 592;
+constexpr int kTable = 512, kSmallTable = 64, kThreads = 256, kPieceBytes = 32768, kVectors = kPieceBytes / (16 * kThreads), kMaxBlocks = 592;
 
 struct Entry {
   const void *in;
@@ -267,6 +267,8 @@ int grad_clip(const void *const *in, void *const *out, const int64_t *numel, con
   double *part = static_cast<double *>(scratch);
   if (total_dtype == T2FW_F64)
     return run<kTable>(in, out, numel, dtype, n, max_norm, static_cast<double *>(total), part, st);
+  // a launch copies its whole table: 15 KB, or 2
+  if (n <= kSmallTable) return run<kSmallTable>(in, out, numel, dtype, n, max_norm, static_cast<float *>(total), part, st);
   return run<kTable>(in, out, numel, dtype, n, max_norm, static_cast<float *>(total), part, st);
 }
 

@@ -1,14 +1,20 @@
-"""GPT-2-small with every attention layer replaced by a fast-weight layer (delta rule or decay rule).
+"""GPT-2-small with every attention layer replaced by a recurrent one: a fast-weight layer (delta rule or decay rule) or a
+gated linear recurrence.
 
 The reference ships the two recurrences but no model around them; this is the caller its
 tests imply: per head, keys are normalised the way tests/test_dfw.py:45-46 builds them
 (softmax over the key dimension times a sigmoid write strength), the decay gate is a sigmoid
 with the positive bias initialisation of tests/test_lfw.py:10-16, and heads are folded into the
 batch dimension ([B, T, H*d] -> [B*H, T, d]) because every batch x head row is an independent
-recurrence.  Everything except the recurrence call is stock PyTorch.
+recurrence.  With rule="glr" a layer is a projection to value and gate, the recurrence over every channel and the output
+projection; with norm="rms" the layer norms become root-mean-square norms that add the residual themselves.  Everything
+except those calls is stock PyTorch.
 
     model = GPT2FW(GPT2FWConfig(rule="dfw")).half().cuda()
     loss = model(token_ids, targets=token_ids)
+
+For inference, `model.eight_bit_()` turns the projections behind the norms (norm="rms", rule "glr" or "lfw") into 8-bit ones:
+the norm then leaves e4m3 values with a scale per row, and the weights have a scale per output.
 
 Data parallelism over several GPUs is torch's DistributedDataParallel (NCCL gradient all-reduce);
 the recurrences themselves need no communication.
@@ -22,7 +28,9 @@ import torch.nn.functional as F
 
 from .functional_dfw import DFWFunction
 from .functional_fused import LFWFusedFunction, unfused_reference
+from .functional_glr import GLRFusedFunction
 from .functional_lfw import LFWFunction
+from .functional_norm import AddRMSNormFunction, RMSNormFunction, add_rms_norm_e4m3, rms_norm_e4m3
 
 
 @dataclass
@@ -32,19 +40,61 @@ class GPT2FWConfig:
     d_model: int = 768
     n_head: int = 12
     n_layer: int = 12
-    rule: str = "dfw"          # "dfw" (delta rule) or "lfw" (decay rule)
+    rule: str = "dfw"          # "dfw" (delta rule), "lfw" (decay rule) or "glr" (gated linear recurrence)
     gate_bias: float = 4.0     # decay gates start near sigmoid(4) = 0.98
+    norm: str = "layer"        # "layer" or "rms"
+    norm_eps: float = 1e-5
+
+
+class Linear8(nn.Module):
+    """An nn.Linear for inference on e4m3 inputs with a scale per row: e4m3 weights with a scale per output."""
+
+    def __init__(self, lin):
+        super().__init__()
+        if lin.weight.dtype not in (torch.float16, torch.bfloat16) or lin.bias is None:
+            raise RuntimeError("8-bit projections are made of fp16 or bf16 ones with a bias")
+        w = lin.weight.detach().float()
+        scale = (w.abs().amax(dim=1, keepdim=True) / 448.0).clamp_min(1e-30)
+        self.register_buffer("weight", (w / scale).to(torch.float8_e4m3fn))
+        self.register_buffer("scale", scale.t().contiguous())
+        self.register_buffer("bias", lin.bias.detach().clone())
+
+    def forward(self, x):
+        q, scale = x
+        y = torch._scaled_mm(q.flatten(0, -2), self.weight.t(), scale_a=scale.flatten(0, -2), scale_b=self.scale, bias=self.bias,
+                             out_dtype=self.bias.dtype)
+        return y.unflatten(0, q.shape[:-1])
+
+
+class RMSNorm(nn.Module):
+    """norm(x) -> y; norm(x, residual) -> (y, x + residual).  With `eight_bit` y is a pair (e4m3 values, scales)."""
+
+    def __init__(self, d, eps):
+        super().__init__()
+        self.weight = nn.Parameter(torch.ones(d))
+        self.eps, self.eight_bit = eps, False
+
+    def forward(self, x, residual=None):
+        if self.eight_bit:
+            if residual is None:
+                return rms_norm_e4m3(x, self.weight, self.eps)
+            q, scale, s = add_rms_norm_e4m3(x, residual, self.weight, self.eps)
+            return (q, scale), s
+        if residual is None:
+            return RMSNormFunction.apply(x, self.weight, self.eps)
+        return AddRMSNormFunction.apply(x, residual, self.weight, self.eps)
 
 
 class FastWeightAttention(nn.Module):
-    """Causal token mixing by a fast-weight memory of shape [d_head, d_head] per head."""
+    """Causal token mixing by a fast-weight memory of shape [d_head, d_head] per head, or by a gated linear recurrence over
+    every channel."""
 
     def __init__(self, cfg):
         super().__init__()
         assert cfg.d_model % cfg.n_head == 0
         self.h, self.d = cfg.n_head, cfg.d_model // cfg.n_head
         self.rule = cfg.rule
-        n_proj = 3 if cfg.rule == "dfw" else 4          # q, k, v (+ key-side decay gate)
+        n_proj = {"dfw": 3, "lfw": 4, "glr": 2}[cfg.rule]      # q, k, v (+ key-side decay gate); value and gate
         self.qkv = nn.Linear(cfg.d_model, n_proj * cfg.d_model)
         if cfg.rule == "dfw":
             self.strength = nn.Linear(cfg.d_model, cfg.n_head)   # write strength per head
@@ -55,14 +105,18 @@ class FastWeightAttention(nn.Module):
         return t.view(B, T, self.h, self.d).permute(0, 2, 1, 3).reshape(B * self.h, T, self.d)
 
     def forward(self, x):
-        B, T, C = x.shape
+        if self.rule == "glr":
+            vg = self.qkv(x)      # value | gate pre-activation
+            out, _ = GLRFusedFunction.apply(vg, vg.new_zeros(vg.shape[0], vg.shape[2] // 2))
+            return self.proj(out)
+        B, T, C = (x[0] if isinstance(x, tuple) else x).shape
         if self.rule == "lfw":
             # projection output = query | key | value | gate; the recurrence reads the heads in place
             # and applies the query scale and the gate activation itself (fused entry point); other
             # head sizes and dtypes take the same layer built from the plain operator
             qkvg = self.qkv(x)
-            state = torch.zeros(B * self.h, self.d, self.d, dtype=x.dtype, device=x.device)
-            if self.d == 64 and x.dtype in (torch.float16, torch.bfloat16) and x.is_cuda:
+            state = torch.zeros(B * self.h, self.d, self.d, dtype=qkvg.dtype, device=qkvg.device)
+            if self.d == 64 and qkvg.dtype in (torch.float16, torch.bfloat16) and qkvg.is_cuda:
                 out, _ = LFWFusedFunction.apply(qkvg, state, self.h)
             else:
                 out, _ = unfused_reference(qkvg, state, self.h)
@@ -80,16 +134,29 @@ class FastWeightAttention(nn.Module):
         return self.proj(out)
 
 
+def _norm(cfg):
+    if cfg.norm not in ("layer", "rms"):
+        raise ValueError("norm must be \"layer\" or \"rms\"")
+    return nn.LayerNorm(cfg.d_model) if cfg.norm == "layer" else RMSNorm(cfg.d_model, cfg.norm_eps)
+
+
 class Block(nn.Module):
     def __init__(self, cfg):
         super().__init__()
-        self.ln1 = nn.LayerNorm(cfg.d_model)
+        self.rms = cfg.norm == "rms"
+        self.ln1 = _norm(cfg)
         self.attn = FastWeightAttention(cfg)
-        self.ln2 = nn.LayerNorm(cfg.d_model)
+        self.ln2 = _norm(cfg)
         self.fc = nn.Linear(cfg.d_model, 4 * cfg.d_model)
         self.out = nn.Linear(4 * cfg.d_model, cfg.d_model)
 
-    def forward(self, x):
+    def forward(self, x, residual=None):
+        """The block's output; with norm="rms" a pair of what the last projection gave and the residual stream, which the next
+        norm adds."""
+        if self.rms:
+            h, x = (self.ln1(x), x) if residual is None else self.ln1(x, residual)
+            h, x = self.ln2(self.attn(h), x)
+            return self.out(F.gelu(self.fc(h), approximate="tanh")), x
         x = x + self.attn(self.ln1(x))
         return x + self.out(F.gelu(self.fc(self.ln2(x)), approximate="tanh"))
 
@@ -104,7 +171,7 @@ class GPT2FW(nn.Module):
         self.wte = nn.Embedding(self.vocab_padded, cfg.d_model)
         self.wpe = nn.Embedding(cfg.n_positions, cfg.d_model)
         self.blocks = nn.ModuleList(Block(cfg) for _ in range(cfg.n_layer))
-        self.ln_f = nn.LayerNorm(cfg.d_model)
+        self.ln_f = _norm(cfg)
         self.apply(self._init)
         for blk in self.blocks:      # GPT-2's scaled init of the residual projections
             for lin in (blk.attn.proj, blk.out):
@@ -112,6 +179,9 @@ class GPT2FW(nn.Module):
             if cfg.rule == "lfw":    # decay gates start near 1 (tests/test_lfw.py:10-16)
                 with torch.no_grad():
                     blk.attn.qkv.bias[3 * cfg.d_model:].fill_(cfg.gate_bias)
+            elif cfg.rule == "glr":
+                with torch.no_grad():
+                    blk.attn.qkv.bias[cfg.d_model:].fill_(cfg.gate_bias)
 
     @staticmethod
     def _init(m):
@@ -125,13 +195,31 @@ class GPT2FW(nn.Module):
     def n_params(self):
         return sum(p.numel() for p in self.parameters())
 
+    def eight_bit_(self):
+        """For inference: the projections behind the norms of the blocks (query | key | value | gate, or value | gate, and the
+        first of the feed-forward layer) become 8-bit ones, their inputs 8-bit outputs of the norms.  Call it on an fp16 or
+        bf16 model, and the model under torch.no_grad()."""
+        if self.cfg.norm != "rms" or self.cfg.rule not in ("glr", "lfw"):
+            raise RuntimeError("8-bit projections need norm=\"rms\" and rule \"glr\" or \"lfw\"")
+        for blk in self.blocks:
+            blk.attn.qkv, blk.fc = Linear8(blk.attn.qkv), Linear8(blk.fc)
+            blk.ln1.eight_bit = blk.ln2.eight_bit = True
+        return self
+
     def forward(self, ids, targets=None):
         B, T = ids.shape
         pos = torch.arange(T, device=ids.device)
         x = self.wte(ids) + self.wpe(pos)
-        for blk in self.blocks:
-            x = blk(x)
-        logits = F.linear(self.ln_f(x), self.wte.weight)          # tied output embedding
+        if self.cfg.norm == "rms":
+            residual = None
+            for blk in self.blocks:
+                x, residual = blk(x, residual)
+            x = self.ln_f(x) if residual is None else self.ln_f(x, residual)[0]
+        else:
+            for blk in self.blocks:
+                x = blk(x)
+            x = self.ln_f(x)
+        logits = F.linear(x, self.wte.weight)          # tied output embedding
         if targets is None:
             return logits
         return F.cross_entropy(logits.view(B * T, -1), targets.reshape(B * T)).float()

@@ -104,3 +104,22 @@ def test_c_clipping_checks_its_lists():
     _fails(call(tdt=0), 1, "norm is float32")
     _fails(call(size=8), 3, "scratch")
     assert lib.t2fw_grad_clip_scratch_bytes(0) == 0
+
+
+def test_model_options_that_do_not_exist():
+    from t2fw_b200.gpt2_fw import GPT2FW, GPT2FWConfig, Linear8
+
+    def _config(rule="glr", norm="rms"):
+        return GPT2FWConfig(vocab_size=200, n_positions=128, d_model=64, n_head=1, n_layer=2, rule=rule, norm=norm)
+
+    for cfg in (_config("dfw"), _config("glr", "layer")):
+        with pytest.raises(RuntimeError, match="8-bit"):
+            GPT2FW(cfg).eight_bit_()
+    with pytest.raises(RuntimeError, match="8-bit"):
+        GPT2FW(_config()).eight_bit_()      # fp32
+    with pytest.raises(RuntimeError, match="8-bit"):
+        Linear8(torch.nn.Linear(4, 4, bias=False).half())
+    with pytest.raises(ValueError, match="norm"):
+        GPT2FW(_config(norm="batch"))
+    with pytest.raises(KeyError):
+        GPT2FW(_config(rule="rnn"))
