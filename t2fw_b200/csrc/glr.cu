@@ -1,5 +1,7 @@
 // The gated linear recurrence: choice of the storage type (kernels in glr_scan.cuh, one file per type), and single steps.
-#include "common.cuh"
+#include <initializer_list>
+
+#include "glr.cuh"
 
 namespace t2fw {
 
@@ -12,23 +14,36 @@ int glr_backward_t(const void *go, const void *gs, const void *x, const void *f,
 
 namespace {
 
-// One step: every array is a flat list of n = B*D numbers.  `state` and `next` may be the same array (an element is read and
-// then written by the same thread), so nothing here is declared free of aliases.
-template <typename T>
+// One step: every array is a flat list of n = B*D numbers, V of them to a thread.  `state` and `next` may be the same array (a
+// thread reads what it then writes), so nothing here is declared free of aliases.
+template <typename T, int V>
 __global__ void __launch_bounds__(256)
 glr_step_kernel(const T *x, const T *f, const T *state, T *out, T *next, int64_t n) {
   using A = typename Elem<T>::acc;
+  using R = typename glr::Raw<T, V>::type;
   dependency_wait();
-  const int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
+  const int64_t i = ((int64_t)blockIdx.x * blockDim.x + threadIdx.x) * V;
   if (i >= n) return;
-  const A h = (A)Elem<T>::ld(f + i) * (A)Elem<T>::ld(state + i) + (A)Elem<T>::ld(x + i);
-  Elem<T>::st(out + i, h);
-  Elem<T>::st(next + i, h);
+  A h[V], fv[V], xv[V];
+  glr::unpack<T, V>(*reinterpret_cast<const R *>(state + i), h);
+  glr::unpack<T, V>(*reinterpret_cast<const R *>(f + i), fv);
+  glr::unpack<T, V>(*reinterpret_cast<const R *>(x + i), xv);
+  glr::fma_v(h, fv, h, xv);
+  const R r = glr::pack<T, V>(h);
+  *reinterpret_cast<R *>(out + i) = r;
+  *reinterpret_cast<R *>(next + i) = r;
 }
 
+// 16 bytes to a thread where the pointers allow it and the threads are many (a small call is over sooner with more of them).
 template <typename T>
 int launch_step(const void *x, const void *f, const void *state, void *out, void *next, int64_t n, cudaStream_t st) {
-  T2FW_CHECK_CUDA(launch_dependent(glr_step_kernel<T>, dim3((unsigned)ceil_div64(n, 256)), dim3(256), 0, st,
+  constexpr int V = 16 / (int)sizeof(T);
+  uintptr_t low = 0;
+  for (const void *q : {x, f, state, static_cast<const void *>(out), static_cast<const void *>(next)}) low |= reinterpret_cast<uintptr_t>(q);
+  const bool wide = n % V == 0 && (low & 15) == 0 && n >= 1 << 18;
+  const int64_t blocks = ceil_div64(wide ? n / V : n, 256);
+  T2FW_CHECK_ARG(blocks <= 0x7fffffff, "sizes out of range");
+  T2FW_CHECK_CUDA(launch_dependent(wide ? glr_step_kernel<T, V> : glr_step_kernel<T, 1>, dim3((unsigned)blocks), dim3(256), 0, st,
                                    static_cast<const T *>(x), static_cast<const T *>(f), static_cast<const T *>(state),
                                    static_cast<T *>(out), static_cast<T *>(next), n));
   T2FW_CHECK_LAUNCH(1);

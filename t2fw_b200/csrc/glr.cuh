@@ -60,40 +60,53 @@ __device__ __forceinline__ typename Raw<T, V>::type pack(const A (&v)[V]) {
   return u;
 }
 
-// e = exp(-g), a = sigmoid(g) = 1 / (1 + e) and rest = 1 - a = e a, each to full relative precision.  -g is held at 80 (700):
-// beyond that a is below 2e-35, and e would overflow.  For 16-bit storage the exponential and the reciprocal are the fast ones:
-// some units of 2^-23, where the result is rounded to 2^-9 or 2^-12.  A NaN stays.
-template <bool kFast>
-__device__ __forceinline__ void gate_pair(float g, float &a, float &rest) {
-  float x, e;
-  asm("min.NaN.f32 %0, %1, %2;" : "=f"(x) : "f"(-g), "f"(80.f));
-  if constexpr (kFast) {
-    e = __expf(x);
-    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(a) : "f"(1.f + e));
-  } else {
-    e = expf(x);
-    a = 1.f / (1.f + e);
-  }
-  rest = e * a;
-}
-template <bool kFast>
-__device__ __forceinline__ void gate_pair(double g, double &a, double &rest) {
-  const double e = exp(-g > 700.0 ? 700.0 : -g);
-  a = 1.0 / (1.0 + e);
-  rest = e * a;
-}
-
-// A run of steps acts on the state as c -> P c + S.  A product P that leaves the range upwards is held at the largest finite
-// number, so that a state of zero stays one (P c is 0, not infinity times zero) and a gate of zero ends what was before.
-// Where the steps themselves would meet an infinity or a NaN, S is none either.
-__device__ __forceinline__ float held(float P) {
-  float r;      // |P| or the limit, whichever is less, with P's sign; a NaN stays
-  asm("min.NaN.xorsign.abs.f32 %0, %1, %2;" : "=f"(r) : "f"(P), "f"(3.402823466e38f));
+// e = exp(-g), a = sigmoid(g) = 1 / (1 + e) and rest = 1 - a = e a, each to full relative precision.  g is held at -80 (-700):
+// below that a is less than 2e-35, and e would overflow.  For 16-bit storage e = 2^(-g log2 e) and the reciprocal are the fast
+// ones: some units of 2^-23, where the result is rounded to 2^-9 or 2^-12.  A NaN stays.
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
   return r;
 }
-__device__ __forceinline__ double held(double P) {
-  return P > 1.7976931348623157e308 ? 1.7976931348623157e308 : P < -1.7976931348623157e308 ? -1.7976931348623157e308 : P;
+template <bool kFast, int V>
+__device__ __forceinline__ void gates(float (&g)[V], float (&rest)[V]) {      // g becomes a
+  if constexpr (kFast) {
+    float e[V];
+#pragma unroll
+    for (int k = 0; k < V; ++k) {
+      const float x = max_nan(g[k], -80.f) * -1.44269504f;      // log2 e: off by less than one unit of 2^-24 of it
+      asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e[k]) : "f"(x));
+    }
+#pragma unroll
+    for (int k = 0; k < V; ++k) asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(g[k]) : "f"(1.f + e[k]));
+#pragma unroll
+    for (int k = 0; k < V; ++k) rest[k] = e[k] * g[k];
+  } else {
+#pragma unroll
+    for (int k = 0; k < V; ++k) {
+      const float e = expf(-max_nan(g[k], -80.f));
+      asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(g[k]) : "f"(1.f + e));      // off by one unit of 2^-23 at most
+      rest[k] = e * g[k];
+    }
+  }
 }
+template <bool kFast, int V>
+__device__ __forceinline__ void gates(double (&g)[V], double (&rest)[V]) {
+#pragma unroll
+  for (int k = 0; k < V; ++k) {
+    const double e = exp(-(g[k] < -700.0 ? -700.0 : g[k]));
+    g[k] = 1.0 / (1.0 + e);
+    rest[k] = e * g[k];
+  }
+}
+
+// A run of steps acts on the state as c -> P c + S.  Products of gates may leave the range upwards; then a state of exactly zero
+// stays what S makes of it, and a product that is exactly zero stays zero, as in the steps one by one; any other state becomes
+// infinite or NaN.  (Where the steps themselves meet an infinity or a NaN, S is none either.)
+template <typename A>
+__device__ __forceinline__ A apply(A P, A S, A c) { return c == A(0) ? S : P * c + S; }
+template <typename A>
+__device__ __forceinline__ A product(A first, A then) { return first == A(0) ? A(0) : first * then; }
 
 // V products, V sums of products: pairs of fp32 in one instruction.
 template <typename A, int V>
@@ -106,6 +119,21 @@ __device__ __forceinline__ void mul_v(A (&r)[V], const A (&a)[V], const A (&b)[V
 #pragma unroll
     for (int k = 0; k < V; ++k) r[k] = a[k] * b[k];
   }
+}
+// Whether all |v| are at most 1: products of such cannot leave the range upwards.  (A NaN is not at most 1.)
+template <int V>
+__device__ __forceinline__ bool tame(const float (&v)[V]) {
+  float m = 0.f;
+#pragma unroll
+  for (int k = 0; k < V; ++k) m = max_nan(m, fabsf(v[k]));
+  return m <= 1.f;
+}
+template <int V>
+__device__ __forceinline__ bool tame(const double (&v)[V]) {
+  bool ok = true;
+#pragma unroll
+  for (int k = 0; k < V; ++k) ok = ok && fabs(v[k]) <= 1.0;
+  return ok;
 }
 template <typename A, int V>
 __device__ __forceinline__ void fma_v(A (&r)[V], const A (&a)[V], const A (&b)[V], const A (&c)[V]) {

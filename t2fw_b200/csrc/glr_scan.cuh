@@ -140,8 +140,7 @@ glr_scan_kernel(const ScanArgs<T> p) {
     unpack<T, V>(raw(it, 0, i), u);
     unpack<T, V>(raw(it, 1, i), f);
     if constexpr (kFused) {
-#pragma unroll
-      for (int k = 0; k < V; ++k) gate_pair<kFast>(f[k], f[k], rest[k]);
+      gates<kFast>(f, rest);
       if constexpr (!kBwd) mul_v(u, u, rest);
     }
   };
@@ -190,8 +189,8 @@ glr_scan_kernel(const ScanArgs<T> p) {
           A Pb = A(1), Sb = A(0);
 #pragma unroll
           for (int w = 0; w < kWarps; ++w) {
-            Sb = m[k][w].x * Sb + m[k][w].y;
-            Pb = held(Pb * m[k][w].x);
+            Sb = apply(m[k][w].x, m[k][w].y, Sb);
+            Pb = product(Pb, m[k][w].x);
           }
           if (lane + 32 * k < CH) {
             const uint32_t at = smem_u32(half + rank * CH + lane + 32 * k), sem = smem_u32(&bar[h]);
@@ -210,7 +209,7 @@ glr_scan_kernel(const ScanArgs<T> p) {
           for (int r = 0; r < kMaxCluster; ++r)
             if (r < C) {
               if (r == rank) start[k] = carry[k];
-              carry[k] = q[r].x * carry[k] + q[r].y;
+              carry[k] = apply(q[r].x, q[r].y, carry[k]);
             }
         }
       }
@@ -219,7 +218,7 @@ glr_scan_kernel(const ScanArgs<T> p) {
 #pragma unroll
         for (int w = 0; w < kWarps; ++w) {
           if (lane + 32 * k < CH) s_in[h][w][lane + 32 * k] = start[k];
-          start[k] = m[k][w].x * start[k] + m[k][w].y;
+          start[k] = apply(m[k][w].x, m[k][w].y, start[k]);
         }
         if (C == 1) carry[k] = start[k];
       }
@@ -244,6 +243,7 @@ glr_scan_kernel(const ScanArgs<T> p) {
     fetch(1);
   }
   A P[V], S[V], P0[V], S0[V];
+  bool calm = true, calm0 = true;
   for (int it = 0;; ++it) {
     if (it < N) {      // A
       if constexpr (kAsync) {
@@ -278,9 +278,8 @@ glr_scan_kernel(const ScanArgs<T> p) {
           }
         }
       }
-#pragma unroll
-      for (int k = 0; k < V; ++k) P[k] = held(P[k]);
       if constexpr (LW < 32) {
+        calm = __all_sync(0xffffffffu, tame(P));      // gates of up to 1, as nearly always: nothing to look out for
 #pragma unroll
         for (int o = LW; o < 32; o <<= 1) {
           A Pp[V], Sp[V];
@@ -290,10 +289,16 @@ glr_scan_kernel(const ScanArgs<T> p) {
             Sp[k] = __shfl_up_sync(0xffffffffu, S[k], o);
           }
           if (lane >= o) {
-            fma_v(S, P, Sp, S);
-            mul_v(P, P, Pp);
+            if (calm) {
+              fma_v(S, P, Sp, S);
+              mul_v(P, P, Pp);
+            } else {
 #pragma unroll
-            for (int k = 0; k < V; ++k) P[k] = held(P[k]);
+              for (int k = 0; k < V; ++k) {
+                S[k] = apply(P[k], S[k], Sp[k]);
+                P[k] = product(Pp[k], P[k]);
+              }
+            }
           }
         }
       }
@@ -313,7 +318,12 @@ glr_scan_kernel(const ScanArgs<T> p) {
       for (int k = 0; k < V; ++k) c[k] = s_in[e & 1][warp][col * V + k];
       if constexpr (LW < 32) {      // what the run before leaves is what enters this one
         A behind[V];
-        fma_v(behind, P0, c, S0);
+        if (calm0) {
+          fma_v(behind, P0, c, S0);
+        } else {
+#pragma unroll
+          for (int k = 0; k < V; ++k) behind[k] = apply(P0[k], S0[k], c[k]);
+        }
 #pragma unroll
         for (int k = 0; k < V; ++k) {
           const A q = __shfl_up_sync(0xffffffffu, behind[k], LW);
@@ -368,6 +378,7 @@ glr_scan_kernel(const ScanArgs<T> p) {
     }
 #pragma unroll
     for (int k = 0; k < V; ++k) P0[k] = P[k], S0[k] = S[k];
+    calm0 = calm;
   }
   copy_wait<0>();
   if (C > 1) cluster_sync();
@@ -426,10 +437,7 @@ glr_walk_kernel(const ScanArgs<T> p, int64_t n) {
         A u[V], f[V], rest[V];
         unpack<T, V>(now[i][0], u);
         unpack<T, V>(now[i][1], f);
-        if constexpr (kFused) {
-#pragma unroll
-          for (int k = 0; k < V; ++k) gate_pair<kFast>(f[k], f[k], rest[k]);
-        }
+        if constexpr (kFused) gates<kFast>(f, rest);
         if constexpr (!kBwd) {
           if constexpr (kFused) mul_v(u, u, rest);
           fma_v(c, f, c, u);
@@ -531,7 +539,8 @@ int launch_v(const ScanArgs<T> &p, int64_t B, cudaStream_t st) {
   // Walkers need many channels or few steps.  Scan against walk, forward, bf16, us: 256 x 64 steps x 768 (24 576 walkers) 20.7 /
   // 16.7, 128 x 64 x 768 11.4 / 13.6, 512 x 128 x 1024 81.0 / 80.8 (backward 131 / 108), 256 x 16 x 768 17.7 / 5.3,
   // 64 x 40 x 768 6.1 / 9.1, 16 x 24 x 512 2.1 / 3.3.
-  if (p.T_ <= 8 || n >= 128 * sms || (n >= 40 * sms && p.T_ <= 32)) {
+  const int64_t full = n * V * (int64_t)sizeof(T) / 16;      // walkers of 16 bytes; narrower ones keep less in flight
+  if (p.T_ <= 8 || full >= 128 * sms || (full >= 40 * sms && p.T_ <= 32)) {
     T2FW_CHECK_ARG(n <= 128 * (int64_t)0x7fffffff, "sizes out of range");
     T2FW_CHECK_CUDA(launch_dependent(glr_walk_kernel<T, V, kFused, kBwd>, dim3((unsigned)ceil_div64(n, 128)), dim3(128), 0, st,
                                      p, n));
@@ -539,13 +548,12 @@ int launch_v(const ScanArgs<T> &p, int64_t B, cudaStream_t st) {
     return T2FW_OK;
   }
   if constexpr (V * sizeof(T) == 16) {
-    constexpr int kMin = kFused && kBwd ? 2 : 3;
     // Full lines, or half lines where those tiles are so few that a cluster each leaves SMs without work.  Full against half,
     // bf16, us, forward and backward: 1 x 65536 x 1024 (16 tiles) 268 / 107 and 324 / 146, 4 x 4096 x 512 (32) 16.1 / 16.6 and
     // 20.9 / 22.0, 64 x 1024 x 1024 76 / 83 and 122 / 130.
     if (B * ceil_div64(p.D, 8 * V) * kMaxCluster >= sms + sms / 2)
-      return launch_scan_v<T, V, 8, kFused, kBwd, 4, 3, 128, kMin>(p, B, sms, st);
-    return launch_scan_v<T, V, 4, kFused, kBwd, 4, 3, 128, kMin>(p, B, sms, st);
+      return launch_scan_v<T, V, 8, kFused, kBwd, 4, 3, 128, kBwd ? 3 : 4>(p, B, sms, st);
+    return launch_scan_v<T, V, 4, kFused, kBwd, 4, 3, 128, 3>(p, B, sms, st);
   } else {
     return launch_scan_v<T, V, 32, kFused, kBwd, 8, 3, 256, 2>(p, B, sms, st);
   }

@@ -17,16 +17,12 @@ namespace t2fw {
 namespace rms {
 
 using glr::Raw;
+using glr::max_nan;
 using glr::pack;
 using glr::unpack;
 
 constexpr float kE4m3Max = 448.f, kMinScale = 1e-30f;
 
-__device__ __forceinline__ float max_nan(float a, float b) {
-  float r;
-  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
-  return r;
-}
 __device__ __forceinline__ float inv_sqrt(float v) { return 1.f / sqrtf(v); }
 __device__ __forceinline__ double inv_sqrt(double v) { return 1.0 / sqrt(v); }
 

@@ -82,7 +82,8 @@ def test_unaligned_tensors(cuda, dtype, offset):
     _check_fused(2, 300, 64, dtype, cuda, "open", 7, offset)
 
 
-@pytest.mark.parametrize("B,T,D", [(1, 12000, 64), (1, 9001, 136), (700, 40, 64), (96, 300, 768), (2, 3000, 2048)])
+@pytest.mark.parametrize("B,T,D", [(1, 12000, 64), (1, 9001, 136), (700, 40, 64), (96, 300, 768), (2, 3000, 2048),
+                                   (40, 400, 501), (30, 100, 1002)])
 def test_larger_grids(cuda, B, T, D):
     _check_plain(B, T, D, torch.bfloat16, cuda, "open", 8)
     _check_fused(B, T, D, torch.bfloat16, cuda, "open", 9)
@@ -159,8 +160,22 @@ def test_zero_states_meet_gates_whose_product_overflows(cuda):
     assert not out[:, :1190].any() and torch.equal(nxt, torch.full_like(nxt, 512.0))
 
 
+def test_no_wrong_finite_numbers_where_products_overflow(cuda):
+    """A tiny state in front of gates whose product leaves the range: what the recurrence gives, or no finite number."""
+    from t2fw_b200.functional_glr import GLRFunction
+
+    for D in (16, 17):
+        f = torch.full((1, 1200, D), 2.0, device=cuda)
+        x, s = torch.zeros_like(f), torch.full((1, D), 2.0 ** -100, device=cuda)
+        out, nxt = GLRFunction.apply(x, f, s)
+        want = torch.tensor([2.0 ** (t - 100) if t < 1000 else float("inf") for t in range(1, 1201)], device=cuda, dtype=torch.float64)
+        assert torch.equal(out[0, :127, 0].double(), want[:127])
+        same = out[0].double() == want[:, None]
+        assert bool((same | ~torch.isfinite(out[0])).all()) and not torch.isfinite(nxt).any()
+
+
 @pytest.mark.parametrize("dtype", DTYPES)
-@pytest.mark.parametrize("B,D", [(1, 1), (3, 77), (256, 768), (1000, 129)])
+@pytest.mark.parametrize("B,D", [(1, 1), (3, 77), (256, 768), (1000, 129), (512, 1024), (513, 1023)])
 def test_decode_steps(cuda, B, D, dtype):
     """Steps into own buffers, the state in place or in turn, against the definition on the state as it was rounded."""
     from t2fw_b200.decode import glr_decode_step
