@@ -295,7 +295,7 @@ int t2fw_selftest_umma16(const float *A1, const float *B1, const float *A2, cons
  * sizes, element-aligned pointers.  The gates are taken as given.  Long sequences are worked on in parts, between which the
  * products of the gates over a part (fp32; fp64 for fp64 storage) carry the state: where such a product leaves the range
  * of its type upwards while the state it meets is no zero, the result is infinite or NaN, which a step-by-step evaluation
- * of gates above 1 reaches soon after.
+ * of gates above 1 reaches soon after; where it leaves it downwards it counts as zero.
  * grad_state may be NULL (zero).
  */
 int t2fw_glr_forward(const void *value, const void *forget, const void *state, void *outputs, void *next_state, int64_t B,

@@ -15,7 +15,8 @@ int glr_backward_t(const void *go, const void *gs, const void *x, const void *f,
 namespace {
 
 // One step: every array is a flat list of n = B*D numbers, V of them to a thread.  `state` and `next` may be the same array (a
-// thread reads what it then writes), so nothing here is declared free of aliases.
+// thread reads what it then writes), so nothing here is declared free of aliases.  A small call is its launch: 256 x 768 takes
+// 3.7 us from Python.
 template <typename T, int V>
 __global__ void __launch_bounds__(256)
 glr_step_kernel(const T *x, const T *f, const T *state, T *out, T *next, int64_t n) {
