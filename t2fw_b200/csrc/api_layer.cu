@@ -100,7 +100,7 @@ int t2fw_rms_norm_backward(const void *grad_y, const void *grad_sum, const void 
     set_error("rms norm backward needs %zu bytes of scratch, got %zu", need, scratch_bytes);
     return T2FW_ERR_SCRATCH;
   }
-  T2FW_CHECK_ARG((reinterpret_cast<uintptr_t>(scratch) & 7) == 0, "scratch must be 8-byte aligned");
+  T2FW_CHECK_ARG((reinterpret_cast<uintptr_t>(scratch) & 15) == 0, "scratch must be 16-byte aligned");
   return rms_norm_backward(grad_y, grad_sum, s, weight, d_s, d_weight, rows, D, eps, dtype, scratch,
                            static_cast<cudaStream_t>(stream));
 }
@@ -126,7 +126,7 @@ static int check_list(const void *const *in, const int64_t *numel, const int *dt
     set_error("gradient norm needs %zu bytes of scratch, got %zu", need, scratch_bytes);
     return T2FW_ERR_SCRATCH;
   }
-  T2FW_CHECK_ARG((reinterpret_cast<uintptr_t>(scratch) & 7) == 0, "scratch must be 8-byte aligned");
+  T2FW_CHECK_ARG((reinterpret_cast<uintptr_t>(scratch) & 15) == 0, "scratch must be 16-byte aligned");
   return T2FW_OK;
 }
 

@@ -222,13 +222,14 @@ rms_bwd_kernel(const BwdArgs<T> p) {
   const int tid = threadIdx.x % GS, group = threadIdx.x / GS;
   const int64_t step = (int64_t)gridDim.x * kRows;
   const A inv_d = A(1) / A(p.D), eps = (A)p.eps;
-  R dy[NV], s[NV], w[kShared ? 1 : NV];
+  constexpr bool kAheadSum = kAhead && NV * sizeof(R) <= 32;      // a third array ahead, where the registers hold it
+  R dy[NV], s[NV], ds_in[NV], w[kShared ? 1 : NV];
   bool on[NV];
   A dw[NV][V];
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
     on[i] = (int64_t)(tid + i * GS) * V < p.D;
-    dy[i] = s[i] = R{};
+    dy[i] = s[i] = ds_in[i] = R{};
 #pragma unroll
     for (int k = 0; k < V; ++k) dw[i][k] = A(0);
   }
@@ -239,6 +240,7 @@ rms_bwd_kernel(const BwdArgs<T> p) {
       if (on[i]) {
         dy[i] = *reinterpret_cast<const R *>(p.dy + at);
         s[i] = *reinterpret_cast<const R *>(p.s + at);
+        if ((kAheadSum || !kAhead) && p.dsum != nullptr) ds_in[i] = *reinterpret_cast<const R *>(p.dsum + at);
       }
     }
   };
@@ -266,9 +268,9 @@ rms_bwd_kernel(const BwdArgs<T> p) {
     R up[NV], cdy[NV], cs[NV];
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      if (p.dsum != nullptr && on[i] && valid)
-        up[i] = *reinterpret_cast<const R *>(p.dsum + row * p.D + (int64_t)(tid + i * GS) * V);
-      cdy[i] = dy[i], cs[i] = s[i];
+      if (kAhead && !kAheadSum && p.dsum != nullptr && on[i] && valid)
+        ds_in[i] = *reinterpret_cast<const R *>(p.dsum + row * p.D + (int64_t)(tid + i * GS) * V);
+      up[i] = ds_in[i], cdy[i] = dy[i], cs[i] = s[i];
     }
     if (kAhead && row + step < p.rows) load(row + step);
     A s2[2] = {A(0), A(0)}, g2[2] = {A(0), A(0)};
@@ -331,8 +333,19 @@ rms_bwd_kernel(const BwdArgs<T> p) {
     for (int i = 0; i < NV; ++i)
       if (on[i]) {
         A *to = p.part + (int64_t)blockIdx.x * p.D + (tid + i * GS) * V;
+        if constexpr (V * sizeof(A) % 16 == 0) {      // 16 bytes at a time: single values of a thread lie 32 bytes from the next one's
+          constexpr int W = 16 / (int)sizeof(A);
 #pragma unroll
-        for (int k = 0; k < V; ++k) to[k] = dw[i][k];
+          for (int k = 0; k < V; k += W) {
+            A part[W];
+#pragma unroll
+            for (int j = 0; j < W; ++j) part[j] = dw[i][k + j];
+            *reinterpret_cast<uint4 *>(to + k) = glr::pack<A, W>(part);
+          }
+        } else {
+#pragma unroll
+          for (int k = 0; k < V; ++k) to[k] = dw[i][k];
+        }
       }
   }
 }
@@ -446,7 +459,8 @@ int launch_fwd_as(const FwdArgs<T> &p, int sms, cudaStream_t st) {
 }
 template <typename T, int V, int NV, int GS>
 int launch_bwd_as(const BwdArgs<T> &p, int sms, int64_t *parts, cudaStream_t st) {
-  *parts = capped(grid_of<GS>(p.rows, sms, blocks_per_sm<GS>() / 2));
+  constexpr int kPer = GS <= 32 && NV == 1 ? 3 : blocks_per_sm<GS>() / 2;
+  *parts = capped(grid_of<GS>(p.rows, sms, kPer));
   T2FW_CHECK_CUDA(launch_dependent(rms_bwd_kernel<T, V, NV, GS>, dim3((unsigned)*parts), dim3(block_of<GS>()), 0, st, p));
   T2FW_CHECK_LAUNCH(1);
   return T2FW_OK;
