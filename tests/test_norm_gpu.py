@@ -9,7 +9,7 @@ pytestmark = pytest.mark.gpu
 EPS = 1e-5
 DTYPES = [torch.float16, torch.bfloat16, torch.float32, torch.float64]
 # (leading sizes, D): single values, around a vector, a warp's row, a block's row, rows beyond what registers hold
-SHAPES = [((1,), 1), ((3,), 7), ((2, 3), 8), ((5,), 100), ((1,), 256), ((300,), 264), ((7,), 768), ((2, 33), 1001), ((1100,), 128),
+SHAPES = [((1,), 1), ((3,), 7), ((2, 3), 8), ((5,), 100), ((1,), 256), ((300,), 264), ((300,), 330), ((5,), 1002), ((3,), 6002), ((7,), 768), ((2, 33), 1001), ((1100,), 128),
           ((9,), 2048), ((3,), 5000), ((2,), 16384), ((3,), 20001), ((1,), 70000), ((2500,), 24)]
 
 
