@@ -9,7 +9,7 @@
 // Bound by memory: a row stays in registers from its one read to its write.  y and q are computed from s before its rounding to
 // the storage type; the gradients read s as it was written, and form rstd anew from it, so nothing else is saved.  Measured, with
 // nothing in L2: 16384 x 2048 fp16 with the residual 45 us forward (91 % of the copy bandwidth), 42 with the 8-bit output (86 %),
-// 49 backward (85 %); 8192 x 768 fp16 8.2 and 15.5 us (the weight gradient's second launch is 2 of them).
+// 47 backward (88 %); 8192 x 768 fp16 8.2 and 15.3 us (the weight gradient's second launch is some 3 of them).
 #pragma once
 
 #include <cuda_fp8.h>

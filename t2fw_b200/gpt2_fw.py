@@ -53,6 +53,8 @@ class Linear8(nn.Module):
         super().__init__()
         if lin.weight.dtype not in (torch.float16, torch.bfloat16) or lin.bias is None:
             raise RuntimeError("8-bit projections are made of fp16 or bf16 ones with a bias")
+        if lin.in_features % 16 or lin.out_features % 16:
+            raise RuntimeError("8-bit projections need sizes that are multiples of 16")
         w = lin.weight.detach().float()
         scale = (w.abs().amax(dim=1, keepdim=True) / 448.0).clamp_min(1e-30)
         self.register_buffer("weight", (w / scale).to(torch.float8_e4m3fn))
@@ -94,6 +96,8 @@ class FastWeightAttention(nn.Module):
         assert cfg.d_model % cfg.n_head == 0
         self.h, self.d = cfg.n_head, cfg.d_model // cfg.n_head
         self.rule = cfg.rule
+        if cfg.rule not in ("dfw", "lfw", "glr"):
+            raise ValueError("rule must be \"dfw\", \"lfw\" or \"glr\"")
         n_proj = {"dfw": 3, "lfw": 4, "glr": 2}[cfg.rule]      # q, k, v (+ key-side decay gate); value and gate
         self.qkv = nn.Linear(cfg.d_model, n_proj * cfg.d_model)
         if cfg.rule == "dfw":
@@ -198,7 +202,7 @@ class GPT2FW(nn.Module):
     def eight_bit_(self):
         """For inference: the projections behind the norms of the blocks (query | key | value | gate, or value | gate, and the
         first of the feed-forward layer) become 8-bit ones, their inputs 8-bit outputs of the norms.  Call it on an fp16 or
-        bf16 model, and the model under torch.no_grad()."""
+        bf16 model that is not cast afterwards, and the model under torch.no_grad()."""
         if self.cfg.norm != "rms" or self.cfg.rule not in ("glr", "lfw"):
             raise RuntimeError("8-bit projections need norm=\"rms\" and rule \"glr\" or \"lfw\"")
         for blk in self.blocks:

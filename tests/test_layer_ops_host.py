@@ -121,5 +121,7 @@ def test_model_options_that_do_not_exist():
         Linear8(torch.nn.Linear(4, 4, bias=False).half())
     with pytest.raises(ValueError, match="norm"):
         GPT2FW(_config(norm="batch"))
-    with pytest.raises(KeyError):
+    with pytest.raises(RuntimeError, match="multiples of 16"):
+        Linear8(torch.nn.Linear(16, 24).half())
+    with pytest.raises(ValueError, match="rule"):
         GPT2FW(_config(rule="rnn"))
