@@ -294,10 +294,22 @@ std::vector<at::Tensor> grad_clip(const std::vector<at::Tensor> &tensors, double
   List l = gather(tensors);
   check_max_norm(max_norm);
   const c10::cuda::CUDAGuard guard(tensors[0].device());
+  // One allocation for all results, each at a multiple of 512 bytes: one from the allocator for each took 21 of 29 us for 28
+  // small tensors.  They are tensors of their own on one storage, not views of one another.
   std::vector<at::Tensor> r(1);
   r.reserve(tensors.size() + 1);
-  for (const at::Tensor &t : tensors)
-    r.emplace_back(at::detail::empty_strided_cuda(t.sizes(), t.strides(), t.scalar_type(), t.device()));
+  size_t bytes = 0;
+  auto room = [](const at::Tensor &t) { return (t.nbytes() + 511) / 512 * 512; };
+  for (const at::Tensor &t : tensors) bytes += room(t);
+  auto *allocator = c10::cuda::CUDACachingAllocator::get();
+  const c10::Storage storage(c10::Storage::use_byte_size_t(), bytes, allocator->allocate(bytes), allocator, /*resizable=*/false);
+  size_t at = 0;
+  for (const at::Tensor &t : tensors) {
+    r.emplace_back(at::detail::make_tensor<c10::TensorImpl>(c10::Storage(storage), c10::DispatchKeySet(c10::DispatchKey::CUDA),
+                                                            t.dtype()));
+    r.back().unsafeGetTensorImpl()->set_sizes_and_strides(t.sizes(), t.strides(), (int64_t)(at / t.itemsize()));
+    at += room(t);
+  }
   for (const int64_t i : l.at) l.out.push_back(r[i + 1].data_ptr());
   r[0] = call(l, tensors[0], max_norm, true);
   return r;

@@ -53,7 +53,8 @@ def clip_grad_norm_(parameters, max_norm, error_if_nonfinite=False):
 
 
 def clip_grads(grads, max_norm):
-    """(list of clipped gradients, norm before).  Not differentiable: a derivative through the result raises."""
+    """(list of clipped gradients, norm before).  The results lie in one allocation, which lives as long as one of them does.
+    Not differentiable: a derivative through the result raises."""
     max_norm = _max_norm(max_norm)
     grads = list(grads)
     if not grads:

@@ -126,6 +126,28 @@ def test_strides_that_cover_their_memory(cuda):
     _check_scaled([o], [g], c)
 
 
+def test_results_are_tensors_of_their_own(cuda):
+    """They share an allocation and nothing else: a change of one, also by autograd's books, is none of the others."""
+    from t2fw_b200.grad_clip import clip_grads
+
+    grads = _grads(DTYPES, cuda, 8)
+    out, _ = clip_grads(grads, 1.0)
+    spans = sorted((o.data_ptr(), o.data_ptr() + o.nbytes) for o in out)
+    assert all(a[1] <= b[0] for a, b in zip(spans, spans[1:])) and all(o.data_ptr() % 512 == 0 for o in out)
+    kept = [o.clone() for o in out]
+    w = torch.ones_like(out[4]).requires_grad_(True)
+    y = (w * out[4]).sum()      # saves a result
+    for i, o in enumerate(out):
+        if i != 4:
+            assert not o._is_view() and o.is_contiguous() and not o.requires_grad
+            o.add_(1.0)
+    y.backward()
+    assert torch.equal(w.grad, kept[4]) and torch.equal(out[4], kept[4])
+    assert torch.equal(out[0], kept[0] + 1.0)
+    del out[1:], y
+    assert torch.equal(torch.clone(out[0]), kept[0] + 1.0) and out[0].to("cpu").shape == grads[0].shape
+
+
 def test_large_tensor(cuda):
     from t2fw_b200.grad_clip import clip_grads, global_norm
 
