@@ -182,21 +182,22 @@ rms_fwd_kernel(const FwdArgs<T> p) {
     A ss = sums[0] + sums[1];
     row_reduce<GS, k8>(ss, top, red[half]);
     const A rstd = inv_sqrt(ss * inv_d + eps);
-    A f = rstd;
+    A unit = A(1);      // 1 / scale, of 1e30 at most: a factor of its own, since rstd / scale leaves the range for rows of (nearly) nothing
     if constexpr (k8) {
       const float scale = max_nan(top * rstd / kE4m3Max, kMinScale);
       if (tid == 0 && valid) p.scale[row] = scale;
-      f = rstd / scale;
+      unit = 1.f / scale;
     }
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       A wv[V];
       unpack<T, V>(w[i], wv);
-      A fv[V];
+      A fv[V], uv[V];
 #pragma unroll
-      for (int k = 0; k < V; ++k) fv[k] = f;
+      for (int k = 0; k < V; ++k) fv[k] = rstd, uv[k] = unit;
       glr::mul_v(s[i], s[i], fv);
       glr::mul_v(s[i], s[i], wv);
+      if constexpr (k8) glr::mul_v(s[i], s[i], uv);
       const int64_t at = row * p.D + (int64_t)(tid + i * GS) * V;
       if (on[i] && valid) {
         if constexpr (k8) *reinterpret_cast<typename Raw8<V>::type *>(static_cast<unsigned char *>(p.q) + at) = pack8<V>(s[i]);
@@ -392,16 +393,17 @@ rms_fwd_long_kernel(const FwdArgs<T> p) {
   }
   row_reduce<512, k8>(ss, top, red);
   const A rstd = inv_sqrt(ss / A(p.D) + (A)p.eps);
-  A f = rstd;
+  A unit = A(1);
   if constexpr (k8) {
     const float scale = max_nan(top * rstd / kE4m3Max, kMinScale);
     if (threadIdx.x == 0) p.scale[blockIdx.x] = scale;
-    f = rstd / scale;
+    unit = 1.f / scale;
   }
   for (int64_t d = threadIdx.x; d < p.D; d += 512) {
     A s = Elem<T>::ld(p.x + base + d);
     if (p.r != nullptr) s += (A)Elem<T>::ld(p.r + base + d);
-    const A v[1] = {s * f * (A)Elem<T>::ld(p.w + d)};
+    A v[1] = {s * rstd * (A)Elem<T>::ld(p.w + d)};
+    if constexpr (k8) v[0] *= unit;
     if constexpr (k8) static_cast<__nv_fp8_storage_t *>(p.q)[base + d] = pack8<1>(v);
     else Elem<T>::st(p.y + base + d, v[0]);
   }

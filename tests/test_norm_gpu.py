@@ -237,3 +237,27 @@ def test_refusals(cuda):
         g, = torch.autograd.grad(cls.apply(x, w, EPS), w, gy, create_graph=True)
         with pytest.raises(RuntimeError, match="not implemented"):
             torch.autograd.grad(g.float().sum(), w)
+
+
+@pytest.mark.parametrize("dtype", DTYPES[:3])
+@pytest.mark.parametrize("D", [8, 96, 1001, 1002, 2048, 70000])
+def test_eight_bit_rows_of_zeros_with_a_tiny_eps(cuda, D, dtype):
+    """y is 0, so q is, however large 1 / sqrt(eps) / scale would be."""
+    from t2fw_b200.functional_norm import add_rms_norm_e4m3, rms_norm_e4m3
+
+    x, w = torch.zeros(3, D, dtype=dtype, device=cuda), torch.ones(D, dtype=dtype, device=cuda)
+    x[1, D // 2] = 1.0
+    for eps in (1e-17, 8e-18, 1e-20, 1e-36):
+        for q, scale in (rms_norm_e4m3(x, w, eps), add_rms_norm_e4m3(x, torch.zeros_like(x), w, eps)[:2]):
+            assert not q[::2].float().any() and torch.equal(scale[::2], torch.full_like(scale[::2], 1e-30))
+            assert float(q[1, D // 2].float()) == 448.0 and int((q[1].float() != 0).sum()) == 1
+
+
+@pytest.mark.parametrize("D", [64, 33, 40000])
+def test_eight_bit_rows_below_the_smallest_scale(cuda, D):
+    """x = 1e-12, w = 1e-30: y is 0.995e-30 and the scale 1e-30; e4m3 holds 0.9375 and 1 there."""
+    from t2fw_b200.functional_norm import rms_norm_e4m3
+
+    x = torch.full((2, D), 1e-12, device=cuda)
+    q, scale = rms_norm_e4m3(x, torch.full((D,), 1e-30, device=cuda), 1e-26)
+    assert torch.equal(scale, torch.full_like(scale, 1e-30)) and bool((q.float() == 1.0).all())
