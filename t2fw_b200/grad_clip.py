@@ -4,8 +4,8 @@
     total = clip_grad_norm_(parameters, max_norm)       # scales the parameters' .grad in place
     clipped, total = clip_grads(grads, max_norm)        # leaves its inputs as they are
 
-Every tensor is multiplied by min(1, max_norm / (total + 1e-6)), the factor of torch.nn.utils.clip_grad_norm_; where that is
-1 the in-place form writes nothing.  Two kernel launches for up to 512 tensors, no synchronisation with the host, sums in
+Every tensor is multiplied by min(1, max_norm / (total + 1e-6)), the factor of torch.nn.utils.clip_grad_norm_, whose arguments
+the in-place form takes in the same places (the 2-norm is the only one); where the factor is 1 it writes nothing.  Two kernel launches for up to 512 tensors, no synchronisation with the host, sums in
 fp64 over vectors of 16 bytes; total is fp32 (fp64 if a tensor is).  A total that is infinite or NaN goes into the factor as it is.  Tensors may be
 of different dtypes; they are dense CUDA tensors of one device, and those that are scaled in place do not share memory.
 """
@@ -32,11 +32,13 @@ def _max_norm(max_norm):
     return max_norm
 
 
-def clip_grad_norm_(parameters, max_norm, error_if_nonfinite=False):
+def clip_grad_norm_(parameters, max_norm, norm_type=2.0, error_if_nonfinite=False):
     """Clips the gradients of `parameters` (a tensor or an iterable of tensors; those without a gradient are passed over) in
-    place and returns their norm before.  error_if_nonfinite waits for the norm on the host and raises before anything is
-    written."""
+    place and returns their norm before.  Any norm_type but 2 is refused.  error_if_nonfinite waits for the norm on the host
+    and raises before anything is written."""
     max_norm = _max_norm(max_norm)
+    if isinstance(norm_type, bool) or float(norm_type) != 2.0:
+        raise ValueError("norm_type must be 2")
     if isinstance(parameters, torch.Tensor):
         parameters = [parameters]
     grads = [p.grad for p in parameters]

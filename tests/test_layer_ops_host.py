@@ -125,3 +125,14 @@ def test_model_options_that_do_not_exist():
         Linear8(torch.nn.Linear(16, 24).half())
     with pytest.raises(ValueError, match="rule"):
         GPT2FW(_config(rule="rnn"))
+
+
+def test_clipping_takes_the_places_of_torchs_arguments():
+    """The third argument is the norm's type, of which there is one, and the fourth asks for an error."""
+    p = torch.nn.Parameter(torch.zeros(3))
+    for bad in (1.0, float("inf"), float("nan"), 0, -2.0, True, False, "inf"):
+        with pytest.raises(ValueError, match="norm_type"):
+            clip_grad_norm_([p], 1.0, bad)
+    for good in (2, 2.0, "2"):
+        assert float(clip_grad_norm_([p], 1.0, good)) == 0 and float(clip_grad_norm_([p], 1.0, good, True)) == 0
+    assert float(clip_grad_norm_([p], 1.0, norm_type=2.0, error_if_nonfinite=True)) == 0
