@@ -294,8 +294,9 @@ int t2fw_selftest_umma16(const float *A1, const float *B1, const float *A2, cons
  * value, forget, outputs and their gradients [B, T, D]; state, next_state and their gradients [B, D].  Every dtype, any
  * sizes, element-aligned pointers.  The gates are taken as given.  Long sequences are worked on in parts, between which the
  * products of the gates over a part (fp32; fp64 for fp64 storage) carry the state: where such a product leaves the range
- * of its type upwards while the state it meets is no zero, the result is infinite or NaN, which a step-by-step evaluation
- * of gates above 1 reaches soon after; where it leaves it downwards it counts as zero.
+ * of its type upwards while the state it meets is no zero, the states behind the part are infinite or NaN, also where those
+ * of an evaluation step by step would be finite (gates above 1 on a tiny state, or with small gates behind them); where it
+ * leaves it downwards it counts as zero.  next_state is the last output, bit for bit.
  * grad_state may be NULL (zero).
  */
 int t2fw_glr_forward(const void *value, const void *forget, const void *state, void *outputs, void *next_state, int64_t B,

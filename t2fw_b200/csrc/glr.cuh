@@ -108,7 +108,11 @@ __device__ __forceinline__ A apply(A P, A S, A c) { return c == A(0) ? S : P * c
 template <typename A>
 __device__ __forceinline__ A product(A first, A then) { return first == A(0) ? A(0) : first * then; }
 
-// V products, V sums of products: pairs of fp32 in one instruction.
+// A sum that is rounded by itself, never merged with the product before it: two walks over the same steps agree.
+__device__ __forceinline__ float add_rn(float a, float b) { return __fadd_rn(a, b); }
+__device__ __forceinline__ double add_rn(double a, double b) { return __dadd_rn(a, b); }
+
+// V products, V sums of products with one rounding each: pairs of fp32 in one instruction.
 template <typename A, int V>
 __device__ __forceinline__ void mul_v(A (&r)[V], const A (&a)[V], const A (&b)[V]) {
   if constexpr (std::is_same<A, float>::value && V % 2 == 0) {
@@ -144,7 +148,7 @@ __device__ __forceinline__ void fma_v(A (&r)[V], const A (&a)[V], const A (&b)[V
                      r[k], r[k + 1]);
   } else {
 #pragma unroll
-    for (int k = 0; k < V; ++k) r[k] = a[k] * b[k] + c[k];
+    for (int k = 0; k < V; ++k) r[k] = fma(a[k], b[k], c[k]);
   }
 }
 

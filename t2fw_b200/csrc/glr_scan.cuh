@@ -39,14 +39,15 @@ struct ScanArgs {
 //   A  every thread composes its steps into one map c -> P c + S, and these are composed over the runs of a warp (shuffles)
 //   B  the maps are composed over the warps of a block (shared memory) and sent to the other blocks of the cluster
 //   C  with the maps of all blocks, what is carried into each warp's steps is known
-//   D  every thread walks its steps again and writes its results
+//   D  every thread walks its steps again and writes its results; who walks the last one writes the final state, so that it is
+//      the last output, rounded from the same number
 // B and C are the work of one more warp.  The others come to D of a round only after A of the next one, so that warp has the
 // time of a round, and they meet it at named barriers: they report their maps and go on, and find what is carried in when they
 // need it.  Maps and carried values alternate between two halves.
 // Each thread copies what it alone will read, `kStages` rounds ahead, so the copies need no barrier.
 //
 // Measured, bf16: 64 x 1024 x 1024 forward 70 us (5.8 TB/s of the bytes that have to move, 88 % of the copy bandwidth), backward
-// 122 (84 %), fused 98 and 152 (63 and 81 %); 1 x 65536 x 1024 109, 149, 147 and 195 us (57, 69, 42 and 63 %).  With many tiles
+// 124 (83 %), fused 99 and 156 (62 and 79 %); 1 x 65536 x 1024 108, 150, 146 and 202 us (57, 69, 42 and 61 %).  With many tiles
 // the instructions bound it: 20 per element where 16 bits are unpacked twice (kept in registers they would halve the warps that
 // fit), half of the issue slots at 15 to 20 warps per SM; fused, two special functions per gate and pass.  With one long row
 // there are 256 blocks, and a round of a block takes 1.6 us, most of it the latency of A and D at two warps per scheduler.
@@ -234,11 +235,6 @@ glr_scan_kernel(const ScanArgs<T> p) {
       report<kThreads + 32>(kIns + h);
     }
     if (gave_up) atomicExch(p.status, 1);
-#pragma unroll
-    for (int k = 0; k < K; ++k) {
-      const int64_t at = d0 + lane + 32 * k;
-      if (rank == 0 && lane + 32 * k < CH && at < D) Elem<T>::st(p.end + b * D + at, carry[k]);
-    }
     if (C > 1) cluster_sync();      // no block leaves while another may still send to it
     return;
   }
@@ -253,6 +249,24 @@ glr_scan_kernel(const ScanArgs<T> p) {
   }
   A P[V], S[V], P0[V], S0[V];
   bool calm = true, calm0 = true;
+  auto enter = [&](int e, A (&c)[V]) {      // what is carried into this thread's steps
+#pragma unroll
+    for (int k = 0; k < V; ++k) c[k] = s_in[e & 1][warp][col * V + k];
+    if constexpr (LW < 32) {      // what the run before leaves is what enters this one
+      A behind[V];
+      if (calm0) {
+        fma_v(behind, P0, c, S0);
+      } else {
+#pragma unroll
+        for (int k = 0; k < V; ++k) behind[k] = apply(P0[k], S0[k], c[k]);
+      }
+#pragma unroll
+      for (int k = 0; k < V; ++k) {
+        const A q = __shfl_up_sync(0xffffffffu, behind[k], LW);
+        if (lane >= LW) c[k] = q;
+      }
+    }
+  };
   for (int it = 0;; ++it) {
     if (it < N) {      // A
       if constexpr (kAsync) {
@@ -323,22 +337,7 @@ glr_scan_kernel(const ScanArgs<T> p) {
       const int left = room(tau_write);
       T *w0 = out0, *w1 = out1;
       A c[V];
-#pragma unroll
-      for (int k = 0; k < V; ++k) c[k] = s_in[e & 1][warp][col * V + k];
-      if constexpr (LW < 32) {      // what the run before leaves is what enters this one
-        A behind[V];
-        if (calm0) {
-          fma_v(behind, P0, c, S0);
-        } else {
-#pragma unroll
-          for (int k = 0; k < V; ++k) behind[k] = apply(P0[k], S0[k], c[k]);
-        }
-#pragma unroll
-        for (int k = 0; k < V; ++k) {
-          const A q = __shfl_up_sync(0xffffffffu, behind[k], LW);
-          if (lane >= LW) c[k] = q;
-        }
-      }
+      enter(e, c);
 #pragma unroll
       for (int i = 0; i < L; ++i) {
         const bool write = i < left;
@@ -352,7 +351,7 @@ glr_scan_kernel(const ScanArgs<T> p) {
           A before[V];
           unpack<T, V>(raw(e, 2, i), before);
 #pragma unroll
-          for (int k = 0; k < V; ++k) u[k] += c[k];      // r
+          for (int k = 0; k < V; ++k) u[k] = add_rn(u[k], c[k]);      // r
           mul_v(c, f, u);
           if constexpr (kFused) {
             A v[V];
@@ -390,6 +389,26 @@ glr_scan_kernel(const ScanArgs<T> p) {
     calm0 = calm;
   }
   copy_wait<0>();
+  // The final state is left by who walked the last step, in the last round.  These steps are walked once more, out here: a store in
+  // the loop above cost the fused backward pass 8 to 10 %.
+  const int left = room(tau_write - hop);
+  if (__any_sync(0xffffffffu, left > 0 && left <= L)) {
+    A c[V];
+    enter(N - 1, c);
+#pragma unroll
+    for (int i = 0; i < L; ++i) {
+      A u[V], f[V], rest[V];
+      values(N - 1, i, u, f, rest);
+      if constexpr (!kBwd) {
+        fma_v(c, f, c, u);
+      } else {
+#pragma unroll
+        for (int k = 0; k < V; ++k) u[k] = add_rn(u[k], c[k]);
+        mul_v(c, f, u);
+      }
+      if (i == left - 1) *reinterpret_cast<R *>(p.end + b * D + d) = pack<T, V>(c);
+    }
+  }
   if (C > 1) cluster_sync();
 }
 

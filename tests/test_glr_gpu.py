@@ -316,3 +316,36 @@ def test_refusals(cuda):
     both = torch.zeros(3, 8, dtype=torch.float16, device=cuda)
     with pytest.raises(RuntimeError, match="state_out"):
         glr_decode_step(one, gate, both[:2], both[1:], out)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("shape", SHAPES + [(8, 1024, 768), (700, 40, 64), (1, 9001, 136), (40, 400, 501)])
+def test_the_final_state_is_the_last_output(cuda, shape, dtype):
+    """Bit for bit, and so is the state's gradient f_1 r_1 where d_value holds r_1 unrounded: who goes on from the state goes on
+    from what was reported."""
+    from t2fw_b200.functional_glr import GLRFunction, GLRFusedFunction
+
+    x, f, s, go, gs, vg = _inputs(*shape, dtype, cuda, "open", 40 + sum(shape))
+    leaves = [t.requires_grad_(True) for t in (x, f, s)]
+    out, nxt = GLRFunction.apply(*leaves)
+    assert torch.equal(nxt, out[:, -1])
+    dx, _, ds = torch.autograd.grad([out, nxt], leaves, [go, gs])
+    if dtype in (torch.float32, torch.float64):
+        assert torch.equal(ds, f[:, 0] * dx[:, 0])
+    out, nxt = GLRFusedFunction.apply(vg, s)
+    assert torch.equal(nxt, out[:, -1])
+
+
+@pytest.mark.parametrize("D", [16, 17])
+def test_a_finite_last_output_is_a_finite_state(cuda, D):
+    """128 gates of 1, then 128 of 2: the product of a part is 2^128, beyond fp32, but no state is."""
+    from t2fw_b200.functional_glr import GLRFunction
+
+    f = torch.ones(1, 256, D, device=cuda)
+    f[:, 128:] = 2.0
+    x, s = torch.zeros_like(f), torch.full((1, D), 2.0 ** -100, device=cuda)
+    out, nxt = GLRFunction.apply(x, f, s)
+    assert torch.equal(nxt, out[:, -1]) and bool((nxt == 2.0 ** 28).all())
+    leaves = [t.requires_grad_(True) for t in (x, f.flip(1).contiguous(), torch.zeros_like(s))]
+    dx, _, ds = torch.autograd.grad(GLRFunction.apply(*leaves)[1], leaves, s)
+    assert bool((dx[:, 0] == 2.0 ** 27).all()) and bool((ds == 2.0 ** 28).all())
