@@ -142,6 +142,8 @@ void glr_decode_step(const at::Tensor &value, const at::Tensor &forget, const at
                   !overlap(outputs, state_out) && !overlap(state_out, value) && !overlap(state_out, forget),
               "outputs and state_out must not share memory with another argument");
   const c10::cuda::CUDAGuard guard(value.device());
+  mark_changed(state_out);
+  mark_changed(outputs);
   check_status(t2fw_glr_forward(value.data_ptr(), forget.data_ptr(), state_in.data_ptr(), outputs.data_ptr(),
                                 state_out.data_ptr(), B, 1, D, dtype_code(value),
                                 at::cuda::getCurrentCUDAStream().stream()),

@@ -43,6 +43,12 @@ inline at::Tensor new_tensor(at::IntArrayRef sizes, at::ScalarType dtype, const 
 }
 inline at::Tensor new_like(const at::Tensor &t) { return new_tensor(t.sizes(), t.scalar_type(), t); }
 
+// For a tensor of the caller's that a kernel is about to write: what saved it for a backward pass is to notice.  (Inference
+// tensors cannot be saved and have no counter.)
+inline void mark_changed(const at::Tensor &t) {
+  if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
+
 // Scratch of one call: freed when the call returns, which the caching allocator orders on the stream.
 inline c10::DataPtr make_scratch(size_t bytes) {
   if (bytes == 0) return c10::DataPtr();

@@ -349,3 +349,34 @@ def test_a_finite_last_output_is_a_finite_state(cuda, D):
     leaves = [t.requires_grad_(True) for t in (x, f.flip(1).contiguous(), torch.zeros_like(s))]
     dx, _, ds = torch.autograd.grad(GLRFunction.apply(*leaves)[1], leaves, s)
     assert bool((dx[:, 0] == 2.0 ** 27).all()) and bool((ds == 2.0 ** 28).all())
+
+
+@pytest.mark.parametrize("native", [True, False])
+def test_a_decode_step_marks_what_it_writes(cuda, native):
+    """A backward pass that saved the state or the outputs' buffer raises instead of reading what a step left there."""
+    from t2fw_b200.decode import glr_decode_step
+    from t2fw_b200.functional_glr import GLRFunction
+
+    step = glr_decode_step if native else torch.ops.glr.decode_step
+    x, f, s, go, _, _ = _inputs(2, 1, 8, torch.float32, cuda, "open", 50)
+    for written in ("state", "outputs"):
+        gate = f.clone().requires_grad_(True)
+        state, out = s.clone(), torch.zeros_like(x)
+        if written == "state":
+            y, _ = GLRFunction.apply(x, gate, state)       # saves the state
+        else:
+            y = gate * out
+        step(x, f, state, state, out)
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            torch.autograd.grad(y, gate, go)
+    state, other, out = s.clone(), s.clone(), torch.zeros_like(x)
+    step(x, f, state, other, out)
+    assert (x._version, f._version, state._version, other._version, out._version) == (0, 0, 0, 1, 1)
+    with pytest.raises(RuntimeError, match="share memory"):
+        step(x, f, state, other, x)
+    assert x._version == 0 and other._version == 1
+    with torch.inference_mode():
+        state, other, out = s.clone(), s.clone(), torch.zeros_like(x)
+    step(x, f, state, other, out)
+    step(x, f, state, state, out)
+    assert torch.equal(state, out[:, 0]) and torch.equal(other, state)
