@@ -139,6 +139,8 @@ void lfw_decode_step(const at::Tensor &x, const at::Tensor &f, const at::Tensor 
   TORCH_CHECK(B > 0 && D > 0 && K > 0, "empty tensors are not supported");
   const c10::cuda::CUDAGuard guard(x.device());
   const int dt = dtype_code(x);
+  mark_changed(state_out);
+  mark_changed(outputs);
   auto stream = at::cuda::getCurrentCUDAStream();
   // T = 1: one checkpoint slot, which is the new state
   check_status(t2fw_lfw_forward(x.data_ptr(), f.data_ptr(), query.data_ptr(), key.data_ptr(), f_key.data_ptr(),
@@ -175,6 +177,8 @@ bool lfw_decode_ring(const at::Tensor &x, const at::Tensor &f, const at::Tensor 
                                        stream.stream());
   if (rc == T2FW_ERR_UNSUPPORTED) return false;
   check_status(rc, "lfw.decode_ring");
+  mark_changed(state);
+  mark_changed(outputs);
   return true;
 }
 

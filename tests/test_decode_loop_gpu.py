@@ -97,3 +97,27 @@ def test_autograd_wrapper_under_graph_capture(cuda):
             assert torch.equal(a, b)
     r_out, _ = fw_oracle.lfw_forward(x, f, q, k, fk, s)
     assert max_rel_err(static[0], r_out) <= OUT_TOL[torch.float16]
+
+
+def test_decode_steps_mark_what_they_write(cuda):
+    """A backward pass that saved one of the buffers raises instead of reading what a step left there."""
+    from t2fw_b200.decode import LFWDecodeLoop, lfw_decode_step
+
+    x, f, q, k, fk, s, _, _ = to_dev(lfw_inputs(2, 1, 64, 64, "sigmoid", 0.3, 95), torch.float16, cuda)
+    for step in (lfw_decode_step, torch.ops.lfw.decode_step):
+        other, out, w = torch.empty_like(s), torch.zeros_like(x), torch.ones_like(x).requires_grad_(True)
+        y = (w * out).sum()
+        step(x, f, q, k, fk, s, other, out)
+        assert (s._version, other._version, out._version) == (0, 1, 1)
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            y.backward()
+        with pytest.raises(RuntimeError, match="alternate two buffers"):
+            step(x, f, q, k, fk, other, other, out)
+        assert (other._version, out._version) == (1, 1)
+    with torch.inference_mode():
+        other, out = torch.empty_like(s), torch.zeros_like(x)
+    lfw_decode_step(x, f, q, k, fk, s, other, out)
+    loop = LFWDecodeLoop(s, ring=2)
+    before = loop.state._version, loop.outputs._version
+    loop.run_ring()
+    assert loop.state._version > before[0] and loop.outputs._version > before[1]
