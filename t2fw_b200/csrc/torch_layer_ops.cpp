@@ -337,7 +337,8 @@ TORCH_LIBRARY(glr, m) {
   m.def("backward", glr_backward);
   m.def("fused_forward", glr_fused_forward);
   m.def("fused_backward", glr_fused_backward);
-  m.def("decode_step", glr_decode_step);
+  m.def("decode_step(Tensor value, Tensor forget, Tensor state_in, Tensor(a!) state_out, Tensor(b!) outputs) -> ()",
+        glr_decode_step);
 }
 
 TORCH_LIBRARY(rms, m) {
@@ -349,5 +350,5 @@ TORCH_LIBRARY(rms, m) {
 TORCH_LIBRARY(gradclip, m) {
   m.def("norm", grad_norm);
   m.def("clip", grad_clip);
-  m.def("clip_", grad_clip_);
+  m.def("clip_(Tensor(a!)[] tensors, float max_norm) -> Tensor", grad_clip_);
 }

@@ -378,7 +378,8 @@ using namespace t2fw_ops;
 TORCH_LIBRARY(lfw, m) {
   m.def("forward", lfw_forward);
   m.def("backward", lfw_backward);
-  m.def("decode_step", lfw_decode_step);
+  m.def("decode_step(Tensor x, Tensor f, Tensor query, Tensor key, Tensor f_key, Tensor state_in, Tensor(a!) state_out, "
+        "Tensor(b!) outputs) -> ()", lfw_decode_step);
   m.def("fused_forward", lfw_fused_forward);
   m.def("fused_backward", lfw_fused_backward);
   m.def("segment_summary", lfw_segment_summary);

@@ -136,3 +136,15 @@ def test_clipping_takes_the_places_of_torchs_arguments():
     for good in (2, 2.0, "2"):
         assert float(clip_grad_norm_([p], 1.0, good)) == 0 and float(clip_grad_norm_([p], 1.0, good, True)) == 0
     assert float(clip_grad_norm_([p], 1.0, norm_type=2.0, error_if_nonfinite=True)) == 0
+
+
+def test_schemas_name_what_is_written():
+    """An operator that returns nothing and is said to write nothing may be dropped or moved by what reads schemas."""
+    for op, written in ((torch.ops.glr.decode_step, {"state_out", "outputs"}), (torch.ops.gradclip.clip_, {"tensors"}),
+                        (torch.ops.lfw.decode_step, {"state_out", "outputs"})):
+        schema = op.default._schema
+        assert schema.is_mutable
+        assert {a.name for a in schema.arguments if a.alias_info is not None and a.alias_info.is_write} == written
+    for op in (torch.ops.glr.forward, torch.ops.glr.fused_backward, torch.ops.rms.backward, torch.ops.rms.e4m3, torch.ops.gradclip.norm,
+               torch.ops.gradclip.clip):
+        assert not op.default._schema.is_mutable
