@@ -53,15 +53,18 @@ __device__ __forceinline__ int find(const Table<N> &t, uint32_t p) {
   return lo;
 }
 
-// Sum of squares of a vector, in fp64.  For a total in fp32, the eight squares of 16-bit values are added in fp32 first (off by
-// 2^-22 at most, each vector another way); where the sum is not well inside fp32's range, which bf16 can leave, in fp64 too.
+// Sum of squares of a vector, in fp64.  For a total in fp32, the eight squares of 16-bit values, each of them exact, are added in
+// fp32 first, in a tree: off by 3 * 2^-24 at most, so a total by half of that and its own rounding (one behind the other they
+// lose up to 7 * 2^-24, always the same way, where one value in eight is large).  Where the sum is not well inside fp32's range,
+// which bf16 can leave, in fp64 too.
 template <typename T>
 __device__ __forceinline__ double squares(const uint4 &u, bool exact) {
   if constexpr (sizeof(T) == 2) {
-    float v[8], q = 0.f;
+    float v[8], p[4];
     glr::unpack<T, 8>(u, v);
 #pragma unroll
-    for (int k = 0; k < 8; ++k) q += v[k] * v[k];
+    for (int k = 0; k < 4; ++k) p[k] = v[2 * k] * v[2 * k] + v[2 * k + 1] * v[2 * k + 1];
+    const float q = (p[0] + p[1]) + (p[2] + p[3]);
     if (!exact && q > 0x1p-90f && q < 0x1p120f) return (double)q;
     if (((u.x | u.y | u.z | u.w) & 0x7fff7fffu) == 0) return 0.0;
     double s = 0;

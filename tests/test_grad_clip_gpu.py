@@ -282,3 +282,18 @@ def test_refusals(cuda):
         with pytest.raises(RuntimeError, match="share memory"):
             clip_grad_norm_(params, 1.0)
     assert torch.equal(g, before)
+
+
+@pytest.mark.parametrize("dtype", DTYPES[:2])
+@pytest.mark.parametrize("place", range(8))
+def test_one_large_value_in_eight(cuda, dtype, place):
+    """The squares of eight neighbours are added in fp32, in three levels: 3 * 2^-24 of their sum, half of that of the norm, which
+    is then rounded (2^-24).  Small values whose squares lie just below half a step of the large one's are where that is reached."""
+    from t2fw_b200.grad_clip import global_norm
+
+    for small in (2.0 ** -12, 2.43e-4, 3.4e-4, 2.0 ** -11, 1e-3):
+        v = torch.full((8,), small, device=cuda)
+        v[place] = 1.0
+        g = v.repeat(4096).to(dtype)
+        ref = g.double().square().sum().sqrt()
+        assert abs(float(global_norm([g])) - float(ref)) <= (2.5 * 2.0 ** -24 + 2.0 ** -40) * float(ref)
