@@ -322,6 +322,8 @@ int t2fw_glr_fused_backward(const void *grad_output, const void *grad_state, con
  *
  * residual and sum are NULL together.  y is computed from s before its rounding to the storage type.  The 8-bit form
  * writes q = e4m3(y / scale), rounded to nearest, and one fp32 scale = max(max|y| / 448, 1e-30) per row; no fp64.
+ * Sums are kept in fp32 (fp64 for fp64 storage); rows whose squares leave that range are summed again from scaled values, so
+ * any finite row is normalised.
  * Backward: `s` is what the forward call left in `sum` (x without a residual); d_s is the gradient of x and of the
  * residual alike; grad_sum, the gradient of `sum` from its other uses, may be NULL (zero).
  */

@@ -8,13 +8,14 @@
 //
 // Bound by memory: a row stays in registers from its one read to its write.  y and q are computed from s before its rounding to
 // the storage type; the gradients read s as it was written, and form rstd anew from it, so nothing else is saved.  Measured, with
-// nothing in L2: 16384 x 2048 fp16 with the residual 45 us forward (91 % of the copy bandwidth), 42 with the 8-bit output (86 %),
+// nothing in L2: 16384 x 2048 fp16 with the residual 45 us forward (91 % of the copy bandwidth), 40 with the 8-bit output (90 %),
 // 47 backward (88 %); 8192 x 768 fp16 8.2 and 15.3 us (the weight gradient's second launch is some 3 of them).
 #pragma once
 
 #include <cuda_fp8.h>
 
 #include <initializer_list>
+#include <type_traits>
 
 #include "glr.cuh"
 
@@ -28,6 +29,7 @@ using glr::unpack;
 
 constexpr float kE4m3Max = 448.f, kMinScale = 1e-30f;
 
+__device__ __forceinline__ double max_nan(double a, double b) { return a > b || a != a ? a : b; }
 __device__ __forceinline__ float inv_sqrt(float v) { return 1.f / sqrtf(v); }
 __device__ __forceinline__ double inv_sqrt(double v) { return 1.0 / sqrt(v); }
 
@@ -58,6 +60,29 @@ __device__ __forceinline__ void row_reduce(A &a, A &b, A (*red)[2]) {
       else b += red[i][1];
     }
   }
+}
+
+// Rows whose squares leave the range of A (bf16 and fp32 reach beyond 2^64, and below 2^-55 where eps is no larger) are done once
+// more, with values that a power of two brings inside, when a block has been through its other rows.  Which they are is told from
+// sums formed in the same order, and the sums of a row are the same in each of its threads, so all decide alike.  fp16 values and
+// sums of two lie between 2^-24 and 2^17: never.  A NaN or an infinity is done again and stays.
+// (In the loop over the rows the same code, skipped, cost 8 % of the 8-bit form's time at 16384 x 2048 bf16, and up to 17 %.)
+template <typename T> constexpr bool kLeaves = !std::is_same<T, __half>::value;
+template <typename A> struct Range;
+template <> struct Range<float> {
+  static constexpr float most = 0x1.fffffep127f, least = 0x1p-110f, large = 0x1p40f, down = 0x1p-100f, up = 0x1p90f;
+};
+template <> struct Range<double> {
+  static constexpr double most = 0x1.fffffffffffffp1023, least = 0x1p-900, large = 0x1p300, down = 0x1p-600, up = 0x1p600;
+};
+template <typename A>
+__device__ __forceinline__ bool strays(A ss, A mean) { return !(ss <= Range<A>::most) || mean < Range<A>::least; }
+// a maximum of products, where zero is no stray
+template <typename A>
+__device__ __forceinline__ bool strays(A v) { return !(v <= Range<A>::most) || (v > A(0) && v < Range<A>::least); }
+template <typename A>
+__device__ __forceinline__ A power(A largest) {
+  return largest >= Range<A>::large ? Range<A>::down : largest <= A(1) / Range<A>::large ? Range<A>::up : A(1);
 }
 
 // V values as e4m3, one behind the other.
@@ -103,7 +128,7 @@ template <int GS> constexpr int block_of() { return GS <= 32 ? 256 : GS; }
 template <typename A, int V>
 __device__ __forceinline__ void add_products(A (&sums)[2], const A (&a)[V], const A (&b)[V]) {
   if constexpr (V == 1) {
-    sums[0] += a[0] * b[0];
+    sums[0] = fma(a[0], b[0], sums[0]);
   } else {
 #pragma unroll
     for (int k = 0; k < V; k += 2) {
@@ -115,13 +140,15 @@ __device__ __forceinline__ void add_products(A (&sums)[2], const A (&a)[V], cons
 
 // A row on GS threads, NV vectors of V elements each, in registers; the next row's values are on their way while a row is
 // reduced.  GS <= 32: several rows in a block, a warp or a part of one each.
+// The 8-bit form of 16-bit rows on 128 or 512 threads is held to the registers with which 8 or 2 blocks fit an SM: 16384 x 2048 bf16
+// 44.9 -> 38.6 us, 4096 x 8192 fp16 45.7 -> 38.5.
 template <typename T, int V, int NV, int GS, bool k8>
-__global__ void __launch_bounds__(block_of<GS>())
+__global__ void __launch_bounds__(block_of<GS>(), k8 && sizeof(T) == 2 && NV * V == 16 ? (GS == 128 ? 8 : GS == 512 ? 2 : 0) : 0)
 rms_fwd_kernel(const FwdArgs<T> p) {
   using A = typename Elem<T>::acc;
   using R = typename Raw<T, V>::type;
   constexpr int kRows = block_of<GS>() / GS;
-  __shared__ A red[2][GS > 32 ? GS / 32 : 1][2];
+  __shared__ A red[kLeaves<T> ? 4 : 2][GS > 32 ? GS / 32 : 1][2];
   dependency_wait();
   const int tid = threadIdx.x % GS;
   const int64_t step = (int64_t)gridDim.x * kRows;
@@ -153,6 +180,7 @@ rms_fwd_kernel(const FwdArgs<T> p) {
 #pragma unroll
   for (int i = 0; i < NV; ++i)
     if (on[i]) w[i] = *reinterpret_cast<const R *>(p.w + (tid + i * GS) * V);
+  bool again = false;
   for (int64_t base = first, half = 0; base < p.rows; base += step, row += step, half ^= 1) {
     A s[NV][V], sums[2] = {A(0), A(0)}, top = A(0);
     valid = row < p.rows;
@@ -181,7 +209,8 @@ rms_fwd_kernel(const FwdArgs<T> p) {
     }
     A ss = sums[0] + sums[1];
     row_reduce<GS, k8>(ss, top, red[half]);
-    const A rstd = inv_sqrt(ss * inv_d + eps);
+    const A mean = ss * inv_d + eps, rstd = inv_sqrt(mean);
+    if constexpr (kLeaves<T>) again |= valid && (strays(ss, mean) || (k8 && strays(top)));
     A unit = A(1);      // 1 / scale, of 1e30 at most: a factor of its own, since rstd / scale leaves the range for rows of (nearly) nothing
     if constexpr (k8) {
       const float scale = max_nan(top * rstd / kE4m3Max, kMinScale);
@@ -205,6 +234,77 @@ rms_fwd_kernel(const FwdArgs<T> p) {
       }
     }
   }
+  if constexpr (kLeaves<T>) {
+    if (GS <= 32 ? !__any_sync(0xffffffffu, again) : !again) return;
+    int turn = 0;
+#pragma unroll 1
+    for (int64_t base = first; base < p.rows; base += step) {
+      row = base + threadIdx.x / GS;
+      valid = row < p.rows;
+      const int64_t at = row * p.D;
+      A none = A(0), most = A(0), sum = A(0);
+      A sums[2] = {A(0), A(0)};
+#pragma unroll 1
+      for (int i = 0; i < NV; ++i) {
+        const int64_t d = (int64_t)(tid + i * GS) * V;
+        if (!valid || d >= p.D) continue;
+        A s[V], t[V];
+        unpack<T, V>(*reinterpret_cast<const R *>(p.x + at + d), s);
+        if (add) {
+          unpack<T, V>(*reinterpret_cast<const R *>(p.r + at + d), t);
+#pragma unroll
+          for (int k = 0; k < V; ++k) s[k] += t[k];
+        }
+        add_products(sums, s, s);
+        if constexpr (k8) {
+          unpack<T, V>(*reinterpret_cast<const R *>(p.w + d), t);
+          glr::mul_v(t, t, s);
+#pragma unroll
+          for (int k = 0; k < V; ++k) most = max_nan(most, fabs(t[k]));
+        }
+      }
+      sum = sums[0] + sums[1];
+      row_reduce<GS, k8>(sum, most, red[2 + (turn ^= 1)]);
+      const bool mine = valid && (strays(sum, sum * inv_d + eps) || (k8 && strays(most)));
+      if (GS <= 32 ? !__any_sync(0xffffffffu, mine) : !mine) continue;
+      const int64_t n = mine ? p.D : 0;
+      auto value = [&](int64_t d) {
+        A v = Elem<T>::ld(p.x + at + d);
+        if (add) v += (A)Elem<T>::ld(p.r + at + d);
+        return v;
+      };
+      most = sum = none = A(0);
+#pragma unroll 1
+      for (int64_t d = tid; d < n; d += GS) most = max_nan(most, fabs(value(d)));
+      row_reduce<GS, true>(none, most, red[2 + (turn ^= 1)]);
+      const A pre = power(most);
+#pragma unroll 1
+      for (int64_t d = tid; d < n; d += GS) {
+        const A v = value(d) * pre;
+        sum += v * v;
+      }
+      row_reduce<GS, false>(sum, none, red[2 + (turn ^= 1)]);
+      const A rstd = inv_sqrt(sum * inv_d + eps * pre * pre);
+      A unit = A(1);
+      if constexpr (k8) {
+        most = none = A(0);
+#pragma unroll 1
+        for (int64_t d = tid; d < n; d += GS) most = max_nan(most, fabs(value(d) * pre * rstd * (A)Elem<T>::ld(p.w + d)));
+        row_reduce<GS, true>(none, most, red[2 + (turn ^= 1)]);
+        const float scale = max_nan(most / kE4m3Max, kMinScale);
+        if (tid == 0 && mine) p.scale[row] = scale;
+        unit = 1.f / scale;
+      }
+#pragma unroll 1
+      for (int64_t v0 = tid * V; v0 < n; v0 += GS * V)      // a thread writes what it has written above
+#pragma unroll 1
+        for (int64_t d = v0; d < v0 + V; ++d) {
+          const A v[1] = {value(d) * pre * rstd * (A)Elem<T>::ld(p.w + d) * unit};
+          if constexpr (k8) static_cast<__nv_fp8_storage_t *>(p.q)[at + d] = pack8<1>(v);
+          else Elem<T>::st(p.y + at + d, v[0]);
+        }
+    }
+  }
 }
 
 // The same for the gradients.  A thread sums the weight gradient of its columns over its rows in registers; a block leaves one
@@ -217,7 +317,7 @@ rms_bwd_kernel(const BwdArgs<T> p) {
   using R = typename Raw<T, V>::type;
   constexpr int kRows = block_of<GS>() / GS, kCols = NV * GS * V;
   constexpr bool kAhead = GS > 32, kShared = GS <= 32 && NV > 2;      // where registers are short the weights lie in shared memory
-  __shared__ A red[2][GS > 32 ? GS / 32 : 1][2];
+  __shared__ A red[kLeaves<T> ? 4 : 2][GS > 32 ? GS / 32 : 1][2];
   __shared__ R s_w[kShared ? NV * GS : 1];
   __shared__ A lines[kRows > 1 ? kRows / 2 : 1][kRows > 1 ? kCols : 1];
   dependency_wait();
@@ -264,6 +364,7 @@ rms_bwd_kernel(const BwdArgs<T> p) {
     if constexpr (kShared) unpack<T, V>(s_w[tid + i * GS], v);
     else unpack<T, V>(w[i], v);
   };
+  bool again = false;
   for (int64_t base = first, half = 0; base < p.rows; base += step, row += step, half ^= 1) {
     const bool valid = row < p.rows;
     if (!kAhead && valid) load(row);
@@ -288,7 +389,13 @@ rms_bwd_kernel(const BwdArgs<T> p) {
     }
     A ss = s2[0] + s2[1], gs = g2[0] + g2[1];
     row_reduce<GS, false>(ss, gs, red[half]);
-    const A rstd = inv_sqrt(ss * inv_d + eps), m = gs * inv_d * rstd * rstd * rstd;
+    const A mean = ss * inv_d + eps;
+    A rstd = inv_sqrt(mean), m = gs * inv_d * rstd * rstd * rstd;
+    if constexpr (kLeaves<T>) {
+      const bool stray = valid && strays(ss, mean);
+      again |= stray;
+      if (stray) rstd = m = A(0);      // nothing for the weight gradient yet
+    }
     if (valid) {
 #pragma unroll
       for (int i = 0; i < NV; ++i) {
@@ -309,6 +416,60 @@ rms_bwd_kernel(const BwdArgs<T> p) {
           for (int k = 0; k < V; ++k) v[k] += u[k];
         }
         if (on[i]) *reinterpret_cast<R *>(p.ds + row * p.D + (int64_t)(tid + i * GS) * V) = pack<T, V>(v);
+      }
+    }
+  }
+  if constexpr (kLeaves<T>) {
+    if (GS <= 32 ? __any_sync(0xffffffffu, again) : again) {
+      int turn = 0;
+#pragma unroll 1
+      for (int64_t base = first; base < p.rows; base += step) {
+        row = base + group;
+        const bool valid = row < p.rows;
+        const int64_t at = row * p.D;
+        A none = A(0), most = A(0), sums[2] = {A(0), A(0)}, dot = A(0);
+#pragma unroll 1
+        for (int i = 0; i < NV; ++i) {
+          const int64_t d = (int64_t)(tid + i * GS) * V;
+          if (!valid || d >= p.D) continue;
+          A sv[V];
+          unpack<T, V>(*reinterpret_cast<const R *>(p.s + at + d), sv);
+          add_products(sums, sv, sv);
+        }
+        A sum = sums[0] + sums[1];
+        row_reduce<GS, false>(sum, none, red[2 + (turn ^= 1)]);
+        const bool mine = valid && strays(sum, sum * inv_d + eps);
+        if (GS <= 32 ? !__any_sync(0xffffffffu, mine) : !mine) continue;
+        const int64_t n = mine ? p.D : 0;
+        sum = none = A(0);
+#pragma unroll 1
+        for (int64_t d = tid; d < n; d += GS) most = max_nan(most, fabs((A)Elem<T>::ld(p.s + at + d)));
+        row_reduce<GS, true>(none, most, red[2 + (turn ^= 1)]);
+        const A pre = power(most);
+#pragma unroll 1
+        for (int64_t d = tid; d < n; d += GS) {
+          const A v = (A)Elem<T>::ld(p.s + at + d) * pre;
+          sum += v * v;
+        }
+        row_reduce<GS, false>(sum, none, red[2 + (turn ^= 1)]);
+        const A rstd = inv_sqrt(sum * inv_d + eps * pre * pre);
+#pragma unroll 1
+        for (int64_t d = tid; d < n; d += GS)
+          dot += (A)Elem<T>::ld(p.dy + at + d) * (A)Elem<T>::ld(p.w + d) * ((A)Elem<T>::ld(p.s + at + d) * pre * rstd);
+        row_reduce<GS, false>(dot, none, red[2 + (turn ^= 1)]);
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+#pragma unroll
+          for (int k = 0; k < V; ++k) {
+            const int64_t d = (int64_t)(tid + i * GS) * V + k;
+            if (d < n) {
+              const A sv = (A)Elem<T>::ld(p.s + at + d) * pre * rstd, g = Elem<T>::ld(p.dy + at + d);
+              A v = (g * (A)Elem<T>::ld(p.w + d) - sv * (dot * inv_d)) * rstd * pre;
+              if (p.dsum != nullptr) v += (A)Elem<T>::ld(p.dsum + at + d);
+              Elem<T>::st(p.ds + at + d, v);
+              dw[i][k] += g * sv;
+            }
+          }
       }
     }
   }
@@ -378,31 +539,51 @@ template <typename T, bool k8>
 __global__ void __launch_bounds__(512)
 rms_fwd_long_kernel(const FwdArgs<T> p) {
   using A = typename Elem<T>::acc;
-  __shared__ A red[16][2];
+  __shared__ A red[4][16][2];
   dependency_wait();
   const int64_t base = (int64_t)blockIdx.x * p.D;
-  A ss = A(0), top = A(0);
-  for (int64_t d = threadIdx.x; d < p.D; d += 512) {
+  auto value = [&](int64_t d) {
     A s = Elem<T>::ld(p.x + base + d);
-    if (p.r != nullptr) {
-      s += (A)Elem<T>::ld(p.r + base + d);
-      Elem<T>::st(p.sum + base + d, s);
-    }
+    if (p.r != nullptr) s += (A)Elem<T>::ld(p.r + base + d);
+    return s;
+  };
+  A ss = A(0), top = A(0), pre = A(1);
+  for (int64_t d = threadIdx.x; d < p.D; d += 512) {
+    const A s = value(d);
+    if (p.r != nullptr) Elem<T>::st(p.sum + base + d, s);
     ss += s * s;
     if constexpr (k8) top = max_nan(top, fabsf(s * (A)Elem<T>::ld(p.w + d)));
   }
-  row_reduce<512, k8>(ss, top, red);
-  const A rstd = inv_sqrt(ss / A(p.D) + (A)p.eps);
+  row_reduce<512, k8>(ss, top, red[0]);
+  const A mean = ss / A(p.D) + (A)p.eps;
+  A rstd = inv_sqrt(mean), y_top = top * rstd;
+  if constexpr (kLeaves<T>) {
+    if (strays(ss, mean) || (k8 && strays(top))) {
+      A sum = A(0), none = A(0), most = A(0);
+      for (int64_t d = threadIdx.x; d < p.D; d += 512) most = max_nan(most, fabs(value(d)));
+      row_reduce<512, true>(none, most, red[1]);
+      pre = power(most);
+      for (int64_t d = threadIdx.x; d < p.D; d += 512) {
+        const A s = value(d) * pre;
+        sum += s * s;
+      }
+      row_reduce<512, false>(sum, none, red[2]);
+      rstd = inv_sqrt(sum / A(p.D) + (A)p.eps * pre * pre);
+      if constexpr (k8) {
+        y_top = A(0);
+        for (int64_t d = threadIdx.x; d < p.D; d += 512) y_top = max_nan(y_top, fabsf(value(d) * pre * rstd * (A)Elem<T>::ld(p.w + d)));
+        row_reduce<512, true>(none, y_top, red[3]);
+      }
+    }
+  }
   A unit = A(1);
   if constexpr (k8) {
-    const float scale = max_nan(top * rstd / kE4m3Max, kMinScale);
+    const float scale = max_nan(y_top / kE4m3Max, kMinScale);
     if (threadIdx.x == 0) p.scale[blockIdx.x] = scale;
     unit = 1.f / scale;
   }
   for (int64_t d = threadIdx.x; d < p.D; d += 512) {
-    A s = Elem<T>::ld(p.x + base + d);
-    if (p.r != nullptr) s += (A)Elem<T>::ld(p.r + base + d);
-    A v[1] = {s * rstd * (A)Elem<T>::ld(p.w + d)};
+    A v[1] = {value(d) * pre * rstd * (A)Elem<T>::ld(p.w + d)};
     if constexpr (k8) v[0] *= unit;
     if constexpr (k8) static_cast<__nv_fp8_storage_t *>(p.q)[base + d] = pack8<1>(v);
     else Elem<T>::st(p.y + base + d, v[0]);
@@ -414,7 +595,7 @@ template <typename T>
 __global__ void __launch_bounds__(512)
 rms_bwd_long_kernel(const BwdArgs<T> p) {
   using A = typename Elem<T>::acc;
-  __shared__ A red[2][16][2];
+  __shared__ A red[5][16][2];
   dependency_wait();
   A *const mine = p.part + (int64_t)blockIdx.x * p.D;
   bool first = true;
@@ -428,13 +609,34 @@ rms_bwd_long_kernel(const BwdArgs<T> p) {
       gs += (A)Elem<T>::ld(p.dy + base + d) * (A)Elem<T>::ld(p.w + d) * sv;
     }
     row_reduce<512, false>(ss, gs, red[half]);
-    const A rstd = inv_sqrt(ss / A(p.D) + (A)p.eps), m = gs / A(p.D) * rstd * rstd;
+    const A ms = ss / A(p.D) + (A)p.eps;
+    A pre = A(1), inner = inv_sqrt(ms), m = gs / A(p.D) * inner;
+    if constexpr (kLeaves<T>) {
+      if (strays(ss, ms)) {
+        A sum = A(0), none = A(0), most = A(0);
+        for (int64_t d = threadIdx.x; d < p.D; d += 512) most = max_nan(most, fabs((A)Elem<T>::ld(p.s + base + d)));
+        row_reduce<512, true>(none, most, red[2]);
+        pre = power(most);
+        for (int64_t d = threadIdx.x; d < p.D; d += 512) {
+          const A sv = (A)Elem<T>::ld(p.s + base + d) * pre;
+          sum += sv * sv;
+        }
+        row_reduce<512, false>(sum, none, red[3]);
+        inner = inv_sqrt(sum / A(p.D) + (A)p.eps * pre * pre);
+        sum = A(0);
+        for (int64_t d = threadIdx.x; d < p.D; d += 512)
+          sum += (A)Elem<T>::ld(p.dy + base + d) * (A)Elem<T>::ld(p.w + d) * ((A)Elem<T>::ld(p.s + base + d) * pre * inner);
+        row_reduce<512, false>(sum, none, red[4]);
+        m = sum / A(p.D);
+      }
+    }
+    const A rstd = pre * inner;
     for (int64_t d = threadIdx.x; d < p.D; d += 512) {
-      const A sv = Elem<T>::ld(p.s + base + d), g = Elem<T>::ld(p.dy + base + d);
+      const A sv = (A)Elem<T>::ld(p.s + base + d) * pre * inner, g = Elem<T>::ld(p.dy + base + d);
       A v = rstd * ((A)Elem<T>::ld(p.w + d) * g - sv * m);
       if (p.dsum != nullptr) v += (A)Elem<T>::ld(p.dsum + base + d);
       Elem<T>::st(p.ds + base + d, v);
-      mine[d] = (first ? A(0) : mine[d]) + g * sv * rstd;
+      mine[d] = (first ? A(0) : mine[d]) + g * sv;
     }
     first = false;
   }
@@ -508,6 +710,12 @@ int launch_bwd_v(const BwdArgs<T> &p, int sms, int64_t *parts, cudaStream_t st) 
   return T2FW_OK;
 }
 
+// A positive eps stays positive in A: a row of zeros has a finite 1 / sqrt(eps).
+template <typename A>
+inline double eps_in(double eps) {
+  return std::is_same<A, float>::value && eps > 0 && eps < 0x1p-149 ? 0x1p-149 : eps;
+}
+
 inline bool aligned(int to, std::initializer_list<const void *> ps) {
   uintptr_t low = 0;
   for (const void *q : ps) low |= reinterpret_cast<uintptr_t>(q);
@@ -521,7 +729,7 @@ int rms_forward_t(const void *x, const void *r, const void *w, void *y, void *q,
                   int64_t D, double eps, cudaStream_t st) {
   constexpr int V = 16 / (int)sizeof(T);
   const rms::FwdArgs<T> p = {static_cast<const T *>(x), static_cast<const T *>(r), static_cast<const T *>(w), static_cast<T *>(y),
-                             static_cast<T *>(sum), q, scale, rows, D, eps};
+                             static_cast<T *>(sum), q, scale, rows, D, rms::eps_in<typename Elem<T>::acc>(eps)};
   int sms = 0;
   const int rc = lfw_chunk_sm_count(&sms);
   if (rc != T2FW_OK) return rc;
@@ -538,7 +746,7 @@ int rms_backward_t(const void *dy, const void *dsum, const void *s, const void *
   using A = typename Elem<T>::acc;
   constexpr int V = 16 / (int)sizeof(T);
   const rms::BwdArgs<T> p = {static_cast<const T *>(dy), static_cast<const T *>(dsum), static_cast<const T *>(s),
-                             static_cast<const T *>(w), static_cast<T *>(ds), static_cast<A *>(scratch), rows, D, eps};
+                             static_cast<const T *>(w), static_cast<T *>(ds), static_cast<A *>(scratch), rows, D, rms::eps_in<A>(eps)};
   int sms = 0;
   int64_t parts = 0;
   int rc = lfw_chunk_sm_count(&sms);

@@ -6,7 +6,8 @@
     s = x + residual ,   y = s / sqrt(mean(s^2) + eps) * weight
 
 x, residual [..., D], weight [D], all of one dtype; gradients for x, residual (the same tensor, as the gradient of a sum is)
-and weight.  y is computed from s before s is rounded to the storage type; the backward pass reads s as it was written.
+and weight.  y is computed from s before s is rounded to the storage type; the backward pass reads s as it was written.  Rows of
+any finite values are normalised, also where their squares leave fp32's range.
 
 For an 8-bit projection behind the norm, without gradients:
 

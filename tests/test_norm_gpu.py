@@ -2,7 +2,7 @@
 import pytest
 import torch
 
-from layer_ref import assert_within, rms_norm, unit
+from layer_ref import TINY, assert_within, rms_norm, unit
 
 pytestmark = pytest.mark.gpu
 
@@ -261,3 +261,71 @@ def test_eight_bit_rows_below_the_smallest_scale(cuda, D):
     x = torch.full((2, D), 1e-12, device=cuda)
     q, scale = rms_norm_e4m3(x, torch.full((D,), 1e-30, device=cuda), 1e-26)
     assert torch.equal(scale, torch.full_like(scale, 1e-30)) and bool((q.float() == 1.0).all())
+
+
+# powers of two that take the squares, and their sums, out of fp32's range (fp64's) but not the values themselves
+FAR = {torch.bfloat16: [63, 64, 100, 118, -50, -56, -64, -100], torch.float32: [63, 64, 100, 118, -50, -56, -64, -100],
+       torch.float64: [511, 512, 700, -440, -460, -512]}
+
+
+@pytest.mark.parametrize("dtype", DTYPES[1:])
+@pytest.mark.parametrize("lead,D", [((5,), 8), ((3,), 7), ((9,), 24), ((5,), 100), ((5,), 264), ((4,), 330), ((3,), 768), ((5,), 1001), ((5,), 1002),
+                                    ((3,), 2048), ((3,), 6002), ((2,), 8192), ((2,), 16384), ((3,), 20001), ((2,), 70000)])
+def test_squares_that_leave_the_range(cuda, lead, D, dtype):
+    """With eps = 0 the norm does not depend on a row's size, and a power of two changes no rounding: y and d_weight are those of
+    the rows at size 1, and d_s is smaller by the power.  Rows of every size lie beside one another.  At 2^118 a d_s of less than
+    2^-8 lies below the smallest normal number, 2^-126: its two last roundings (the product with 1 / rms and the sum with gs or the
+    storage type) are then off by half of the smallest subnormal each, 2^118 times as much at size 1."""
+    from t2fw_b200.functional_norm import AddRMSNormFunction, RMSNormFunction
+
+    x, res, w, gy, gs = _inputs(lead, D, dtype, cuda, D + 20)
+    powers = FAR[dtype]
+    big = lambda t, f: (t.detach().double() * f).to(dtype)  # noqa: E731
+    for shift in range(len(powers)):
+        far = [0 if i % 3 == 1 else powers[(i + shift) % len(powers)] for i in range(lead[0])]
+        up = torch.tensor([[2.0 ** k] for k in far], device=cuda, dtype=torch.float64)      # the host's powers are exact, pow() here is not
+        down = 1.0 / up
+        leaves = [t.requires_grad_(True) for t in (big(x, up), big(res, up), w.detach().clone())]
+        assert torch.equal(leaves[0].double(), x.double() * up)
+        y, s = AddRMSNormFunction.apply(*leaves, 0.0)
+        dx, dr, dw = torch.autograd.grad([y, s], leaves, [gy, big(gs, down)])
+        ref = rms_norm(x, res, w, 0.0, gy, gs, dtype)
+        ref["d_s"] = (ref["d_s"][0], ref["d_s"][1] + 2 * TINY[dtype] * up)
+        for name, got in (("y", y), ("sum", s.double() * down), ("d_s", dx.double() * up), ("d_s", dr.double() * up), ("d_weight", dw)):
+            assert_within(got, *ref[name], "add " + name)
+        y = RMSNormFunction.apply(leaves[0], leaves[2], 0.0)
+        dx, dw = torch.autograd.grad(y, [leaves[0], leaves[2]], gy)
+        ref = rms_norm(x, None, w, 0.0, gy, None, dtype)
+        ref["d_s"] = (ref["d_s"][0], ref["d_s"][1] + 2 * TINY[dtype] * up)
+        for name, got in (("y", y), ("d_s", dx.double() * up), ("d_weight", dw)):
+            assert_within(got, *ref[name], name)
+        for i in range(lead[0]):      # a row is what it is alone, whatever lies beside it
+            assert torch.equal(RMSNormFunction.apply(leaves[0][i:i + 1], leaves[2], 0.0)[0], y[i])
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("lead,D", [((5,), 8), ((5,), 100), ((5,), 264), ((3,), 768), ((5,), 1001), ((3,), 2048), ((2,), 16384), ((3,), 20001)])
+def test_eight_bit_rows_of_any_size(cuda, lead, D, dtype):
+    """The same for the 8-bit form; and weights that take the products s w, which y never is, out of the range."""
+    from t2fw_b200.functional_norm import add_rms_norm_e4m3
+
+    x, res, w, _, _ = _inputs(lead, D, dtype, cuda, D + 21)
+    s = x.double() + res.double()
+    y = s / torch.sqrt(s.square().mean(-1, keepdim=True)) * w.double()
+    k = (D / 32 + 26) * unit(dtype)
+    for kx, kw in ((0, 0), (64, 0), (118, 0), (-56, 0), (-100, 0), (30, 100), (118, 100), (-50, -90), (-100, -60)):
+        q, scale, _ = add_rms_norm_e4m3((x.double() * 2.0 ** kx).to(dtype), (res.double() * 2.0 ** kx).to(dtype),
+                                        (w.double() * 2.0 ** kw).to(dtype), 0.0)
+        want = (y.abs().amax(-1, keepdim=True) / 448 * 2.0 ** kw).clamp_min(1e-30)
+        assert_within(scale, want, k * want, "scale %d %d" % (kx, kw))
+        v = y * 2.0 ** kw / scale.double()
+        assert_within(q.double(), v, 2.0 ** -4 * v.abs().clamp_min(2.0 ** -6) + 2 * k * v.abs(), "q %d %d" % (kx, kw))
+
+
+def test_the_smallest_eps_is_not_zero(cuda):
+    from t2fw_b200.functional_norm import RMSNormFunction, rms_norm_e4m3
+
+    for dtype in DTYPES[:3]:
+        for D in (64, 1001, 70000):
+            x, w = torch.zeros(2, D, dtype=dtype, device=cuda), torch.ones(D, dtype=dtype, device=cuda)
+            assert not RMSNormFunction.apply(x, w, 1e-60).any() and not rms_norm_e4m3(x, w, 1e-60)[0].float().any()
