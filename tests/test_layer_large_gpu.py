@@ -118,3 +118,39 @@ def test_first_calls_of_a_process_inside_a_capture(cuda, env):
     r = subprocess.run([sys.executable, "-c", FIRST], cwd=ROOT, env=dict(os.environ, **env), capture_output=True, text=True,
                        timeout=240)
     assert r.returncode == 0 and "equal" in r.stdout, r.stderr[-2000:]
+
+
+@pytest.mark.parametrize("B,T,D", [(1, 1050000, 2056), (3, 1450001, 503)])
+def test_fused_recurrence(cuda, B, T, D):
+    """Gates of sigmoid(0) = 1/2 and values of 2 everywhere, rows of 2 D: the numbers of test_recurrence again."""
+    from t2fw_b200.functional_glr import GLRFusedFunction
+
+    assert B * T * D > 2 ** 31
+    vg = torch.zeros(B, T, 2 * D, dtype=torch.bfloat16, device=cuda)
+    vg[..., :D] = 2.0
+    s = torch.full((B, D), 2.0, dtype=torch.bfloat16, device=cuda)
+    for b, t, d in ((0, 0, 1), (B - 1, T - 2, D - 1), (B - 1, T - 5, 0)):
+        vg[b, t, d] = 18.0
+    leaves = [vg.requires_grad_(True), s.requires_grad_(True)]
+    out, nxt = GLRFusedFunction.apply(*leaves)
+    assert torch.equal(nxt, out[:, -1])
+    dvg, ds = torch.autograd.grad(out, leaves, torch.ones_like(out))
+    n = 12
+    for b in {0, B - 1}:
+        xs, h, first, last = 0.5 * vg[b, :, :D].detach(), s[b].detach().double(), [], []
+        for t in range(n):
+            h = 0.5 * h + xs[t].double()
+            first.append(h)
+        assert torch.equal(out[b, :n].double(), torch.stack(first).bfloat16().double())
+        h = torch.full((D,), 2.0, device=cuda, dtype=torch.float64)
+        for t in range(T - n, T):
+            h = 0.5 * h + xs[t].double()
+            last.append(h)
+        assert torch.equal(out[b, T - n:].double(), torch.stack(last).bfloat16().double())
+        for t in (*range(n), *range(T - n, T)):
+            r = 2.0 - 2.0 ** (t - T + 1) if t >= T - 60 else 2.0
+            before = (out[b, t - 1] if t else s[b]).double()
+            want = torch.cat([torch.full_like(before, 0.5 * r), 0.25 * r * (before - vg[b, t, :D].double())])
+            assert bool(((dvg[b, t].double() - want).abs() <= 2.0 ** -8 * want.abs() + 2.0 ** -20).all())
+        del xs
+    assert bool((ds.double() - 1.0).abs().max() <= 2.0 ** -8)

@@ -131,3 +131,78 @@ def test_eight_bit_model_runs(cuda, rule):
     assert got.shape == (2, 50, 256) and torch.isfinite(got).all()
     with pytest.raises(RuntimeError, match="no gradients"):
         copy.deepcopy(model).eight_bit_()(ids)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("rows", [1, 32, 1000, 8192])
+def test_eight_bit_linear_at_the_models_sizes(cuda, rows, dtype):
+    """d_model to the widths behind the norms: value | gate, and query | key | value | gate or the feed-forward layer's first."""
+    from t2fw_b200.functional_norm import rms_norm_e4m3
+    from t2fw_b200.gpt2_fw import GPT2FWConfig, Linear8
+
+    d = GPT2FWConfig().d_model
+    torch.manual_seed(7)
+    x = torch.randn(rows, d, device=cuda).to(dtype)
+    with torch.no_grad():
+        q, s = rms_norm_e4m3(x, 1 + 0.1 * torch.randn(d, device=cuda).to(dtype), 1e-5)
+    for out in (2 * d, 4 * d):
+        lin8 = Linear8(torch.nn.Linear(d, out).to(cuda, dtype))
+        with torch.no_grad():
+            y = lin8((q, s))
+        assert y.dtype == dtype and y.shape == (rows, out)
+        _check_product(y, q, s, lin8)
+
+
+def _check_product(y, q, s, lin8):
+    """y against 64-bit products of the same 8-bit values: those of two 4-bit significands are exact, their fp32 sum, the two
+    scales and the bias are not, d + 4 roundings."""
+    w = lin8.weight.double() * lin8.scale.double().t()
+    a = q.double().flatten(0, -2) * s.double().flatten(0, -2)
+    ref = a @ w.t() + lin8.bias.double()
+    mag = a.abs() @ w.abs().t() + lin8.bias.double().abs()
+    tol = torch.finfo(y.dtype).eps / 2 * ref.abs() + (q.shape[-1] + 6) * 2.0 ** -24 * mag + 2.0 ** -24
+    assert_within(y.flatten(0, -2), ref, tol)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("rule", ["glr", "lfw"])
+def test_eight_bit_model_at_full_width(cuda, rule, dtype):
+    """Every 8-bit norm and projection inside the model, on what it was given there: the norm against its definition, the product
+    against 64 bits.  And a model that is cast behind eight_bit_() raises."""
+    from t2fw_b200.gpt2_fw import GPT2FW, GPT2FWConfig
+
+    torch.manual_seed(8)
+    model = GPT2FW(GPT2FWConfig(vocab_size=500, n_positions=256, n_layer=2, rule=rule, norm="rms")).to(cuda, dtype)
+    for p in model.parameters():
+        p.data.add_(0.02 * torch.randn_like(p))
+    model.eight_bit_()
+    seen = []
+
+    def norm_hook(m, args, out):
+        x, residual = args[0], args[1] if len(args) > 1 else None
+        (q, scale), s = (out[0], out[1]) if residual is not None else (out, None)
+        total = x.double() + (0 if residual is None else residual.double())
+        if s is not None:
+            assert_within(s, total, (torch.finfo(dtype).eps / 2 + 2.0 ** -23) * total.abs() + 2.0 ** -25)
+        y = total / torch.sqrt(total.square().mean(-1, keepdim=True) + m.eps) * m.weight.double()
+        k = (x.shape[-1] / 32 + 26) * 2.0 ** -24
+        want = (y.abs().amax(-1, keepdim=True) / 448).clamp_min(1e-30)
+        assert_within(scale, want, k * want)
+        v = y / scale.double()
+        assert_within(q.double(), v, 2.0 ** -4 * v.abs().clamp_min(2.0 ** -6) + 2 * k * v.abs())
+        seen.append("norm")
+
+    def product_hook(m, args, out):
+        _check_product(out, *args[0], m)
+        seen.append("product")
+
+    for blk in model.blocks:
+        for m, hook in ((blk.ln1, norm_hook), (blk.ln2, norm_hook), (blk.attn.qkv, product_hook), (blk.fc, product_hook)):
+            m.register_forward_hook(hook)
+    ids = torch.randint(0, 500, (2, 130), device=cuda)
+    with torch.no_grad():
+        logits = model(ids)
+    assert torch.isfinite(logits).all() and sorted(seen) == ["norm"] * 4 + ["product"] * 4
+    other = torch.bfloat16 if dtype == torch.float16 else torch.float16
+    with torch.no_grad(), pytest.raises(RuntimeError):
+        model.to(other)(ids)
