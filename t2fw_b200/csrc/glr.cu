@@ -35,7 +35,9 @@ glr_step_kernel(const T *x, const T *f, const T *state, T *out, T *next, int64_t
   *reinterpret_cast<R *>(next + i) = r;
 }
 
-// 16 bytes to a thread where the pointers allow it and the threads are many (a small call is over sooner with more of them).
+// 16 bytes to a thread where the pointers allow it and the threads are many (a small call is over sooner with more of them).  Single
+// elements against vectors, fp16, us on the device: 65 536 numbers 1.0 / 1.4, 196 608 1.1 / 1.4, 262 144 1.3 / 1.4, 1 M 5.4 / 3.1; in fp32
+// 0.97 / 1.25, 1.86 / 1.85, 2.24 / 2.20, 5.6 / 4.9.
 template <typename T>
 int launch_step(const void *x, const void *f, const void *state, void *out, void *next, int64_t n, cudaStream_t st) {
   constexpr int V = 16 / (int)sizeof(T);

@@ -5,10 +5,9 @@
 // Two launches.  The first leaves one partial sum per block; the second adds them up in each block, in the same order, and
 // scales.  The tensors' addresses and sizes travel as kernel arguments, so a call needs no table in device memory and can be
 // captured.  Work is cut into pieces of 32 KB that begin at 16-byte boundaries, whatever the tensor's own address; a block takes
-// consecutive ones.  Bound by memory: the sums take one conversion to
-// fp64 per vector of 16-bit values, per value in fp32; the second launch walks backwards, from what is still in L2.  Measured on
-// 70 M values: norm 25 us in 16 bits and 45 in fp32 (85 and 96 % of the copy bandwidth), clipped copy 71 and 145 us (three
-// passes over the data: 90 and 89 %).
+// consecutive ones.  Bound by memory: the sums take one conversion to fp64 per vector of 16-bit values, per value in fp32; the
+// second launch walks backwards, from what is still in L2.  Measured on 70 M values: norm 26 us in 16 bits and 45 in fp32 (82 and
+// 95 % of the copy bandwidth), clipped copy 71 and 145 us (three passes over the data: 90 and 89 %).
 #include "glr.cuh"
 
 namespace t2fw {
@@ -17,6 +16,8 @@ namespace {
 
 constexpr int kTable = 512, kSmallTable = 64, kThreads = 256, kPieceBytes = 32768, kVectors = kPieceBytes / (16 * kThreads), kMaxBlocks = 592;
 
+// At most four blocks for each of 148 SMs, as many as fit at once: 70 M bf16 values, norm and clipped copy, us: with half of them
+// 32 / 84, with 592 26.3 / 71.4, with twice as many 26.4 / 69.9, but 10 M fp32 values in place 13.6 instead of 11.7.
 struct Entry {
   const void *in;
   void *out;
@@ -187,6 +188,8 @@ grad_norm_kernel(const __grid_constant__ Table<N> t, double *__restrict__ part, 
 }
 
 // max_norm < 0: only the norm is wanted.
+// Four blocks to an SM leave 64 registers, with which the element-by-element ends spill 80 bytes; with three blocks nothing spills, and
+// 70 M bf16 values take 78 us instead of 71.
 template <int N, typename C>
 __global__ void __launch_bounds__(kThreads, 4)
 grad_scale_kernel(const __grid_constant__ Table<N> t, const double *__restrict__ part, int n_part, double max_norm,
@@ -273,7 +276,7 @@ int grad_clip(const void *const *in, void *const *out, const int64_t *numel, con
   double *part = static_cast<double *>(scratch);
   if (total_dtype == T2FW_F64)
     return run<kTable>(in, out, numel, dtype, n, max_norm, static_cast<double *>(total), part, st);
-  // a launch copies its whole table: 15 KB, or 2
+  // a launch copies its whole table, 15 KB or 2: 28 small tensors 6.3 and 6.2 us on the device
   if (n <= kSmallTable) return run<kSmallTable>(in, out, numel, dtype, n, max_norm, static_cast<float *>(total), part, st);
   return run<kTable>(in, out, numel, dtype, n, max_norm, static_cast<float *>(total), part, st);
 }

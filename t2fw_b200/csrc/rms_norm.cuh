@@ -671,7 +671,11 @@ int launch_bwd_as(const BwdArgs<T> &p, int sms, int64_t *parts, cudaStream_t st)
   return T2FW_OK;
 }
 
-// A row on as few threads as hold it: a part of a warp, a warp, four, eight or sixteen.
+// A row on as few threads as hold it: a part of a warp, a warp, four, eight or sixteen.  fp16, with the residual, us.  Forward, two
+// vectors on a warp against one on 128 threads: 16384 x 264 8.1 / 13.6, 16384 x 512 10.1 / 13.4; against four on a warp, two of them
+// empty, 10.7 and 11.5; three against one on 128 threads: 16384 x 768 15.9 / 17.9; four: 16384 x 1024 20.6 / 22.7.  Few rows would
+// rather have the threads (64 x 1024 2.1 / 1.4).  Backward, two on a warp against one on 128 threads: 16384 x 264 13.8 / 23.7,
+// 16384 x 512 15.3 / 25.1; one on 128 threads against two, half of them empty: 16384 x 768 28.4 / 31.6.
 template <typename T, int V, bool k8>
 int launch_fwd_v(const FwdArgs<T> &p, int sms, cudaStream_t st) {
   const int64_t n = ceil_div64(p.D, V);

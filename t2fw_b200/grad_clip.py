@@ -55,7 +55,8 @@ def clip_grad_norm_(parameters, max_norm, norm_type=2.0, error_if_nonfinite=Fals
 
 
 def clip_grads(grads, max_norm):
-    """(list of clipped gradients, norm before).  The results lie in one allocation, which lives as long as one of them does.
+    """(list of clipped gradients, norm before).  The results lie in one allocation, which lives as long as one of them does and
+    is what torch.save writes for any of them: clone a result that is kept or saved by itself.
     Not differentiable: a derivative through the result raises."""
     max_norm = _max_norm(max_norm)
     grads = list(grads)
