@@ -30,7 +30,8 @@ def lfw_decode_step(x, f, query, key, f_key, state_in, state_out, outputs):
 
 def glr_decode_step(value, forget, state_in, state_out, outputs):
     """h' = forget h + value, the gated linear recurrence's step; writes `outputs` [B,1,D] and `state_out` [B,D].
-    `state_out` may be `state_in`: an element is read and written by the same thread."""
+    `state_out` may be `state_in`: an element is read and written by the same thread.  Both are marked as changed: a backward
+    pass that saved one of them raises."""
     if _ops.glr_step(value, forget, state_in, state_out, outputs) is NotImplemented:
         torch.ops.glr.decode_step(value, forget, state_in, state_out, outputs)
     return outputs, state_out

@@ -2,7 +2,7 @@
 
     outputs, next_state = GLRFunction.apply(value, forget, state)
 
-    h_t = forget_t * h_{t-1} + value_t ,   outputs_t = h_t ,   next_state = h_T
+    h_t = forget_t * h_{t-1} + value_t ,   outputs_t = h_t ,   next_state = h_T = outputs[:, -1], bit for bit
 
 value, forget, outputs [B, T, D]; state, next_state [B, D]; gradients for all three inputs.  It is what the decay rule
 (`LFWFunction`) becomes with a key and a query of one element, and like there the gates are taken as given.
