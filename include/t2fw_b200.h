@@ -324,6 +324,7 @@ int t2fw_glr_fused_backward(const void *grad_output, const void *grad_state, con
  * writes q = e4m3(y / scale), rounded to nearest, and one fp32 scale = max(max|y| / 448, 1e-30) per row; no fp64.
  * Sums are kept in fp32 (fp64 for fp64 storage); rows whose squares leave that range are summed again from scaled values, so
  * any finite row is normalised.
+ * What is written shares no memory with what is read.
  * Backward: `s` is what the forward call left in `sum` (x without a residual); d_s is the gradient of x and of the
  * residual alike; grad_sum, the gradient of `sum` from its other uses, may be NULL (zero).
  */

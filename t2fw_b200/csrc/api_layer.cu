@@ -1,5 +1,7 @@
 // C ABI of the operators that stand around the recurrences in a model (declared in include/t2fw_b200.h): the gated linear
 // recurrence, the root-mean-square norm, gradient clipping.  Argument checks only; nothing here allocates, frees or synchronises.
+#include <initializer_list>
+
 #include "common.cuh"
 
 using namespace t2fw;
@@ -62,12 +64,31 @@ static int check_rms(int64_t rows, int64_t D, double eps, int dtype) {
   return T2FW_OK;
 }
 
+// What is written shares no byte with what is read: rows whose squares leave the range are read again after a first write, and rows
+// that no registers hold are read twice.
+struct Span {
+  const void *p;
+  int64_t bytes;
+};
+static int check_apart(std::initializer_list<Span> out, std::initializer_list<Span> in) {
+  for (const Span &o : out)
+    for (const Span &i : in) {
+      const uintptr_t a = reinterpret_cast<uintptr_t>(o.p), b = reinterpret_cast<uintptr_t>(i.p);
+      T2FW_CHECK_ARG(a == 0 || b == 0 || a >= b + (uint64_t)i.bytes || b >= a + (uint64_t)o.bytes,
+                     "an output shares memory with an input");
+    }
+  return T2FW_OK;
+}
+
 int t2fw_rms_norm_forward(const void *x, const void *residual, const void *weight, void *y, void *sum, int64_t rows,
                           int64_t D, double eps, int dtype, void *stream) {
   const int rc = check_rms(rows, D, eps, dtype);
   if (rc != T2FW_OK) return rc;
   T2FW_CHECK_ARG(x && weight && y, "null pointer argument");
   T2FW_CHECK_ARG((residual == nullptr) == (sum == nullptr), "residual and sum are given together");
+  const int64_t e = (int64_t)dtype_size(dtype), n = rows * D * e;
+  const int apart = check_apart({{y, n}, {sum, n}}, {{x, n}, {residual, n}, {weight, D * e}});
+  if (apart != T2FW_OK) return apart;
   return rms_norm_forward(x, residual, weight, y, sum, rows, D, eps, dtype, static_cast<cudaStream_t>(stream));
 }
 
@@ -81,6 +102,9 @@ int t2fw_rms_norm_e4m3(const void *x, const void *residual, const void *weight, 
     set_error("rms norm with an 8-bit output: 16- and 32-bit storage only");
     return T2FW_ERR_UNSUPPORTED;
   }
+  const int64_t e = (int64_t)dtype_size(dtype), n = rows * D * e;
+  const int apart = check_apart({{q, rows * D}, {scale, rows * 4}, {sum, n}}, {{x, n}, {residual, n}, {weight, D * e}});
+  if (apart != T2FW_OK) return apart;
   return rms_norm_e4m3(x, residual, weight, q, scale, sum, rows, D, eps, dtype, static_cast<cudaStream_t>(stream));
 }
 
@@ -101,6 +125,10 @@ int t2fw_rms_norm_backward(const void *grad_y, const void *grad_sum, const void 
     return T2FW_ERR_SCRATCH;
   }
   T2FW_CHECK_ARG((reinterpret_cast<uintptr_t>(scratch) & 15) == 0, "scratch must be 16-byte aligned");
+  const int64_t e = (int64_t)dtype_size(dtype), n = rows * D * e;
+  const int apart = check_apart({{d_s, n}, {d_weight, D * e}, {scratch, (int64_t)need}},
+                                {{grad_y, n}, {grad_sum, n}, {s, n}, {weight, D * e}});
+  if (apart != T2FW_OK) return apart;
   return rms_norm_backward(grad_y, grad_sum, s, weight, d_s, d_weight, rows, D, eps, dtype, scratch,
                            static_cast<cudaStream_t>(stream));
 }

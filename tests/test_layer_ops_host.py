@@ -148,3 +148,18 @@ def test_schemas_name_what_is_written():
     for op in (torch.ops.glr.forward, torch.ops.glr.fused_backward, torch.ops.rms.backward, torch.ops.rms.e4m3, torch.ops.gradclip.norm,
                torch.ops.gradclip.clip):
         assert not op.default._schema.is_mutable
+
+
+def test_c_norm_refuses_outputs_over_inputs():
+    """A row may be read again after a first write.  (Sizes that no call here gets to work on: the check comes before any CUDA call.)"""
+    lib = _lib.load_core()
+    x, r, w, y, s = (k << 20 for k in range(1, 6))
+    text = "shares memory"
+    for bad in ((x, r, w, x, s), (x, r, w, y, r), (x, r, w, y, x), (x, r, w, x + 62, s), (x, r, w, y, r - 62), (x, r, w, w, s)):
+        _fails(lib.t2fw_rms_norm_forward(*bad, 4, 8, 0.0, 0, None), 1, text)
+    _fails(lib.t2fw_rms_norm_forward(x, None, w, x, None, 4, 8, 0.0, 0, None), 1, text)
+    _fails(lib.t2fw_rms_norm_e4m3(x, r, w, r + 63, y, s, 4, 8, 0.0, 0, None), 1, text)
+    _fails(lib.t2fw_rms_norm_e4m3(x, r, w, y, w, s, 4, 8, 0.0, 0, None), 1, text)
+    size = lib.t2fw_rms_norm_backward_scratch_bytes(4, 8, 0)
+    for d_s, d_w, scratch in ((x, y, s), (r, y, s), (y, w, s), (y, s, x - size + 16)):
+        _fails(lib.t2fw_rms_norm_backward(x, r, 7 << 20, w, d_s, d_w, 4, 8, 0.0, 0, scratch, size, None), 1, text)
